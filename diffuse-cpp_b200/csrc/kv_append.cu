@@ -1,0 +1,475 @@
+// kv_append.cu — dmoe_kv_append: QK norm, rotation and the write of keys and values into a paged
+// cache, with the rotated queries as output.
+//
+// Reference: the fused QKV's split, QK norm and RoPE of src/diffuse-moe-graph.cpp:126-161. For a
+// row x of a query or key head: y = x / sqrt(mean x^2 + eps) * w, then (y_i, y_{i + r/2}) turns by
+// theta_i = position * base^(-2i / r) for i < r / 2. The angle is taken in turns in 64 bits and only its
+// fraction rounded to 32 (at position 131072 a 32-bit angle is already 0.004 off).
+//
+// Pages of 8 bits: for each (32-position block, head) e = the smallest exponent with amax <= 448 * 2^e,
+// and e4m3(x * 2^-e) is stored. A power of two as scale loses nothing against any other scale (e4m3
+// keeps 4 significant bits at every size) and makes the move of kept values to a new scale exact.
+//
+// Work unit: a 32-position block of one sequence that gains rows (the grid is an upper bound of their
+// number, and every warp finds its unit by a scan of the batch). gridDim.y divides the heads: first the
+// groups of heads whose rows are independent (queries; keys and values too in 16-bit pages), then, for
+// 8-bit pages, the groups of key / value heads, where the CTA holds a block of one head in registers
+// until its amax is known. 16 lanes (head_dim 128) or 8 (64) share a row, 8 elements each: 16-byte
+// loads of 16-bit rows, two or four rows a warp at once, and half the shuffles of a warp per row.
+#include <algorithm>
+#include <cmath>
+#include <cstdio>
+
+#include "dmoe_internal.h"
+#include "kv_common.cuh"
+
+namespace dmoe {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr int kMaxHalf = 64;  // rotary_dim / 2 at head_dim 128
+
+struct AppendParams {
+  KvPages pg;
+  KvBatch b;
+  const void* qkv;
+  void* q_out;
+  const float* q_norm;
+  const float* k_norm;
+  int64_t qkv_stride, q_stride;
+  int qkv_type, q_type;
+  int n_head;
+  int half;          // rotary_dim / 2
+  int flat_slots;    // heads of the independent rows: [0, flat_slots)
+  int flat_per_cta, flat_groups, held_per_cta;
+  int vec_in, vec_out;  // rows are 16-byte aligned
+  float eps;
+  double turns[kMaxHalf];  // base^(-2i / rotary_dim) / 2 pi
+};
+
+// 8 consecutive elements as floats. Every type is a vector of 16-byte loads when `vec`.
+__device__ __forceinline__ void load8(const void* p, int64_t at, int type, int vec, float (&x)[8]) {
+  if (type == DMOE_TYPE_F32) {
+    const float* f = static_cast<const float*>(p) + at;
+    if (vec) {
+      const float4 a = __ldcs(reinterpret_cast<const float4*>(f)), b = __ldcs(reinterpret_cast<const float4*>(f) + 1);
+      x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = __ldcs(f + i);
+    }
+    return;
+  }
+  uint32_t w[4];
+  const uint16_t* h = static_cast<const uint16_t*>(p) + at;
+  if (vec) {
+    const uint4 a = __ldcs(reinterpret_cast<const uint4*>(h));
+    w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __ldcs(h + 2 * i) | ((uint32_t)__ldcs(h + 2 * i + 1) << 16);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (type == DMOE_TYPE_F16) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      x[2 * i] = f.x, x[2 * i + 1] = f.y;
+    } else {
+      x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+}
+
+__device__ __forceinline__ uint4 pack8(const float (&x)[8], int type) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (type == DMOE_TYPE_F16) {
+      const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+__device__ __forceinline__ void store8(void* p, int64_t at, int type, int vec, const float (&x)[8]) {
+  if (type == DMOE_TYPE_F32) {
+    float* f = static_cast<float*>(p) + at;
+    if (vec) {
+      reinterpret_cast<float4*>(f)[0] = make_float4(x[0], x[1], x[2], x[3]);
+      reinterpret_cast<float4*>(f)[1] = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = x[i];
+    }
+    return;
+  }
+  const uint4 w = pack8(x, type);
+  uint16_t* h = static_cast<uint16_t*>(p) + at;
+  if (vec) {
+    *reinterpret_cast<uint4*>(h) = w;
+  } else {
+    const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) h[i] = (uint16_t)(v[i / 2] >> (16 * (i & 1)));
+  }
+}
+
+// y = norm(x) * w, then the rotation; every lane of the warp takes part (LPR lanes hold one row).
+// cs: the row's (cos, sin) pairs.
+template <int LPR>
+__device__ __forceinline__ void norm_rotate(float (&x)[8], const float* __restrict__ w, bool norm, float eps, int sub,
+                                            int half, const float2* cs) {
+  float ss = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
+#pragma unroll
+  for (int o = LPR / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  if (norm) {
+    const float r = 1.0f / sqrtf(ss * (1.0f / (8 * LPR)) + eps);
+    const float4 a = __ldg(reinterpret_cast<const float4*>(w) + 2 * sub), b = __ldg(reinterpret_cast<const float4*>(w) + 2 * sub + 1);
+    x[0] *= r * a.x, x[1] *= r * a.y, x[2] *= r * a.z, x[3] *= r * a.w;
+    x[4] *= r * b.x, x[5] *= r * b.y, x[6] *= r * b.z, x[7] *= r * b.w;
+  }
+  if (half == 0) return;
+  const int hl = half / 8;
+  const bool lo = sub < hl, in = sub < 2 * hl;
+  const int lane = threadIdx.x & 31, from = lane + (lo ? hl : in ? -hl : 0);
+  const float2* c = cs + 8 * (lo ? sub : in ? sub - hl : 0);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float y = __shfl_sync(0xffffffffu, x[i], from);
+    const float2 t = c[i];
+    if (in) x[i] = lo ? x[i] * t.x - y * t.y : x[i] * t.x + y * t.y;
+  }
+}
+
+// Scale exponent of a block: amax = f 2^x with 1 <= f < 2, and 448 = 1.75 * 2^8.
+__device__ __forceinline__ int scale_exponent(float amax) {
+  const uint32_t u = __float_as_uint(amax);
+  const int e = (int)(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return min(max(e, kExpMin), kExpMax);  // zero and subnormal amax: the smallest
+}
+
+__device__ __forceinline__ uint2 quantise8(const float (&x)[8], float inv) {
+  uint32_t w[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    uint32_t o = 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float2 f = make_float2(x[4 * j + 2 * i] * inv, x[4 * j + 2 * i + 1] * inv);
+      uint32_t h = __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3);  // round to nearest even
+      if (!(fabsf(f.x) < INFINITY)) h = (h & 0xff00u) | 0x7fu;  // no infinity in e4m3: NaN
+      if (!(fabsf(f.y) < INFINITY)) h = (h & 0x00ffu) | 0x7f00u;
+      o |= h << (16 * i);
+    }
+    w[j] = o;
+  }
+  return make_uint2(w[0], w[1]);
+}
+
+__device__ __forceinline__ void dequantise8(uint2 w, float scale, float (&x)[8]) {
+  const uint32_t v[2] = {w.x, w.y};
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(v[j] >> (16 * i)), __NV_E4M3);
+      const float2 f = __half22float2(__half2(h));
+      x[4 * j + 2 * i] = f.x * scale, x[4 * j + 2 * i + 1] = f.y * scale;
+    }
+}
+
+template <int HD, int KV>
+__global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_constant__ AppendParams p) {
+  constexpr int LPR = HD / 8;     // lanes a row
+  constexpr int RPW = 32 / LPR;   // rows a warp holds at once
+  constexpr int PASSES = kScaleBlock / (kWarps * RPW);
+  __shared__ float2 cs[kScaleBlock * kMaxHalf];
+  __shared__ float amax_s[2][kWarps];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, sub = lane % LPR;
+
+  // this CTA's unit: block `rel` among those of sequence `s` that gain rows
+  int s = -1, rel = (int)blockIdx.x;
+  KvSeq q{};
+  for (int base = 0; base < p.b.n_seq; base += 32) {
+    KvSeq t{};
+    int nb = 0;
+    if (base + lane < p.b.n_seq) {
+      t = kv_sequence(p.b, p.pg, base + lane);
+      const int p0 = max(0, t.kv_len - t.q_len);
+      if (t.q_len > 0) nb = t.kv_len > p0 ? (t.kv_len - 1) / kScaleBlock - p0 / kScaleBlock + 1 : 1;
+    }
+    int sum = nb;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += v;
+    }
+    const uint32_t hit = __ballot_sync(0xffffffffu, sum > rel);
+    if (hit) {
+      const int l = __ffs(hit) - 1;
+      rel -= __shfl_sync(0xffffffffu, sum - nb, l);
+      q.row0 = __shfl_sync(0xffffffffu, t.row0, l);
+      q.q_len = __shfl_sync(0xffffffffu, t.q_len, l);
+      q.kv_len = __shfl_sync(0xffffffffu, t.kv_len, l);
+      s = base + l;
+      break;
+    }
+    rel -= __shfl_sync(0xffffffffu, sum, 31);
+  }
+  if (s < 0) return;
+  const int pos0 = q.kv_len - q.q_len;  // position of the sequence's first row; negative: padding rows
+  const int b0 = (max(0, pos0) / kScaleBlock + rel) * kScaleBlock;
+  const int lo = max(b0, pos0), hi = min(b0 + kScaleBlock, q.kv_len);  // positions that are written
+  const int fresh = max(0, hi - lo);
+  int64_t page = -1;
+  if (fresh > 0) {
+    page = p.b.table[s * p.b.max_pages + b0 / p.pg.page_size];
+    if (page < 0 || page >= p.pg.n_pages) {
+      kv_report(p.pg.err, DMOE_KV_ERR_PAGE);
+      page = -1;
+    }
+  }
+  const int off0 = b0 % p.pg.page_size;
+  const int64_t row_lo = (int64_t)q.row0 + (lo - pos0);  // row of position lo
+  const int group = (int)blockIdx.y;
+
+  // (cos, sin) of the block's new positions, once for all heads of the CTA
+  for (int i = tid; i < fresh * p.half; i += kThreads) {
+    const int t = i / p.half, f = i % p.half;
+    const double a = (double)(lo + t) * p.turns[f];
+    float sn, c;
+    sincospif(2.0f * (float)(a - rint(a)), &sn, &c);
+    cs[(lo - b0 + t) * kMaxHalf + f] = make_float2(c, sn);
+  }
+  __syncthreads();
+
+  if (group < p.flat_groups) {
+    const int h0 = group * p.flat_per_cta, nh = min(p.flat_per_cta, p.flat_slots - h0);
+    if (rel == 0 && pos0 < 0) {  // padding rows: zero queries
+      const int pad = min(-pos0, q.q_len);
+      const float zero[8] = {};
+      for (int r = tid; r < pad * nh * LPR; r += kThreads) {
+        const int h = h0 + (r / LPR) % nh;
+        if (h < p.n_head)
+          store8(p.q_out, (int64_t)(q.row0 + r / LPR / nh) * p.q_stride + (int64_t)h * HD + 8 * (r % LPR), p.q_type,
+                 p.vec_out, zero);
+      }
+    }
+    for (int r0 = warp * RPW; r0 < fresh * nh; r0 += kWarps * RPW) {
+      const int r = r0 + lane / LPR;
+      const bool live = r < fresh * nh;
+      const int t = live ? r % fresh : 0, h = h0 + (live ? r / fresh : 0);
+      float x[8] = {};
+      if (live) load8(p.qkv, (row_lo + t) * p.qkv_stride + (int64_t)h * HD + 8 * sub, p.qkv_type, p.vec_in, x);
+      const float2* c = cs + (lo - b0 + t) * kMaxHalf;
+      if (KV == KV_E4M3) {
+        norm_rotate<LPR>(x, p.q_norm, p.q_norm != nullptr, p.eps, sub, p.half, c);
+        if (live) store8(p.q_out, (row_lo + t) * p.q_stride + (int64_t)h * HD + 8 * sub, p.q_type, p.vec_out, x);
+      } else {
+        const bool is_q = h < p.n_head, is_v = h >= p.n_head + p.pg.n_head_kv;
+        float y[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = x[i];
+        const float* w = is_q ? p.q_norm : p.k_norm;
+        norm_rotate<LPR>(y, w, w != nullptr && !is_v, p.eps, sub, p.half, c);
+        if (!live) continue;
+        if (is_q) {
+          store8(p.q_out, (row_lo + t) * p.q_stride + (int64_t)h * HD + 8 * sub, p.q_type, p.vec_out, y);
+        } else if (page >= 0) {
+          const int hk = is_v ? h - p.n_head - p.pg.n_head_kv : h - p.n_head;
+          const int64_t at = kv_row(p.pg, page, hk, off0 + (lo - b0) + t) * HD + 8 * sub;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) y[i] = is_v ? x[i] : y[i];
+          store8(is_v ? p.pg.v : p.pg.k, at, KV == KV_BF16 ? DMOE_TYPE_BF16 : DMOE_TYPE_F16, 1, y);
+        }
+      }
+    }
+    return;
+  }
+  if (KV != KV_E4M3 || fresh == 0 || page < 0) return;
+
+  const int hs0 = (group - p.flat_groups) * p.held_per_cta, hs1 = min(hs0 + p.held_per_cta, 2 * p.pg.n_head_kv);
+  for (int hs = hs0; hs < hs1; ++hs) {
+    const bool is_v = hs >= p.pg.n_head_kv;
+    const int hk = is_v ? hs - p.pg.n_head_kv : hs;
+    uint8_t* codes = static_cast<uint8_t*>(is_v ? p.pg.v : p.pg.k);
+    uint8_t* sc = (is_v ? p.pg.v_scale : p.pg.k_scale) +
+                  ((page * p.pg.n_head_kv + hk) * p.pg.page_size + off0) / kScaleBlock;
+    const int e_old = lo > b0 ? (int)*sc - 127 : kExpMin;
+    float x[PASSES][8];
+    float amax = 0.f;
+#pragma unroll
+    for (int j = 0; j < PASSES; ++j) {
+      const int t = (j * kWarps + warp) * RPW + lane / LPR, pos = b0 + t;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[j][i] = 0.f;
+      if (pos >= lo && pos < hi) {
+        load8(p.qkv, (row_lo + (pos - lo)) * p.qkv_stride + (int64_t)(p.n_head + hs) * HD + 8 * sub, p.qkv_type,
+              p.vec_in, x[j]);
+      } else if (pos < lo) {
+        const uint2 w = *reinterpret_cast<const uint2*>(codes + kv_row(p.pg, page, hk, off0 + t) * HD + 8 * sub);
+        dequantise8(w, exp2f((float)e_old), x[j]);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < PASSES; ++j) {
+      const int t = (j * kWarps + warp) * RPW + lane / LPR;
+      if (!is_v) {  // uniform over the CTA; rows that are kept pass through
+        float y[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = x[j][i];
+        const bool now = b0 + t >= lo && b0 + t < hi;
+        norm_rotate<LPR>(y, p.k_norm, p.k_norm != nullptr, p.eps, sub, p.half, cs + (now ? t : lo - b0) * kMaxHalf);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[j][i] = now ? y[i] : x[j][i];
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float a = fabsf(x[j][i]);
+        amax = fmaxf(amax, a < INFINITY ? a : 0.f);
+      }
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    if (lane == 0) amax_s[hs & 1][warp] = amax;
+    __syncthreads();  // also: every thread has read the old scale
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) amax = fmaxf(amax, amax_s[hs & 1][w]);
+    const int e = scale_exponent(amax);
+    const float inv = exp2f((float)-e);
+#pragma unroll
+    for (int j = 0; j < PASSES; ++j) {
+      const int t = (j * kWarps + warp) * RPW + lane / LPR, pos = b0 + t;
+      if (pos < hi && (pos >= lo || e != e_old))
+        *reinterpret_cast<uint2*>(codes + kv_row(p.pg, page, hk, off0 + t) * HD + 8 * sub) = quantise8(x[j], inv);
+    }
+    if (tid == 0) *sc = (uint8_t)(e + 127);
+  }
+}
+
+bool is_float_type(int t) { return t == DMOE_TYPE_F32 || t == DMOE_TYPE_F16 || t == DMOE_TYPE_BF16; }
+int64_t size_of(int t) { return t == DMOE_TYPE_F32 ? 4 : 2; }
+bool aligned16(const void* p, int64_t stride_bytes) {
+  return ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)stride_bytes) & 15u) == 0;
+}
+
+}  // namespace
+
+dmoe_status kv_check(const char* call, const dmoe_kv_cache* c, const dmoe_kv_batch* b, int64_t n_tokens, int n_head) {
+  char msg[256];
+  auto fail = [&](dmoe_status st, const char* what) {
+    snprintf(msg, sizeof(msg), "%s: %s", call, what);
+    set_last_error(msg);
+    return st;
+  };
+  if (!c || !b) return fail(DMOE_ERR_INVALID_ARG, "null pointer");
+  if (n_tokens < 0 || n_tokens > INT32_MAX || b->n_seq < 0 || b->max_q_len < 0 || b->max_pages < 0)
+    return fail(DMOE_ERR_INVALID_ARG, "negative size, or 2^31 tokens or more");
+  if (c->type != DMOE_TYPE_BF16 && c->type != DMOE_TYPE_F16 && c->type != DMOE_TYPE_E4M3)
+    return fail(DMOE_ERR_UNSUPPORTED, "pages are bf16, f16 or e4m3");
+  if (c->head_dim != 64 && c->head_dim != 128) return fail(DMOE_ERR_UNSUPPORTED, "head_dim must be 64 or 128");
+  if (c->n_head_kv <= 0 || n_head <= 0 || n_head % c->n_head_kv || n_head > 4096)
+    return fail(DMOE_ERR_INVALID_ARG, "n_head must be a multiple of n_head_kv, at most 4096");
+  if (c->page_size <= 0 || c->page_size % kScaleBlock || c->page_size > 65536)
+    return fail(DMOE_ERR_UNSUPPORTED, "page_size must be a multiple of 32, at most 65536");
+  if (c->n_pages <= 0 || c->n_pages > INT32_MAX) return fail(DMOE_ERR_INVALID_ARG, "n_pages must be in [1, 2^31)");
+  if (b->max_pages > (1 << 30) / c->page_size)
+    return fail(DMOE_ERR_UNSUPPORTED, "max_pages * page_size must be at most 2^30");
+  if (!c->k || !c->v || (c->type == DMOE_TYPE_E4M3 && (!c->k_scale || !c->v_scale)))
+    return fail(DMOE_ERR_INVALID_ARG, "null pointer in the cache");
+  if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15u)
+    return fail(DMOE_ERR_INVALID_ARG, "k and v must be 16-byte aligned");
+  if (b->n_seq > 0 && n_tokens > 0 && (!b->q_start || !b->kv_len || (b->max_pages > 0 && !b->page_table)))
+    return fail(DMOE_ERR_INVALID_ARG, "null pointer in the batch");
+  if ((reinterpret_cast<uintptr_t>(b->q_start) | reinterpret_cast<uintptr_t>(b->kv_len) |
+       reinterpret_cast<uintptr_t>(b->page_table) | reinterpret_cast<uintptr_t>(c->err)) & 3u)
+    return fail(DMOE_ERR_INVALID_ARG, "q_start, kv_len, page_table and err must be 4-byte aligned");
+  return DMOE_OK;
+}
+
+}  // namespace dmoe
+
+using namespace dmoe;
+
+extern "C" dmoe_status dmoe_kv_append(const dmoe_kv_cache* cache, const dmoe_kv_batch* batch,
+                                      const dmoe_kv_append_args* a, void* stream) {
+  auto fail = [](dmoe_status st, const char* what) {
+    char msg[320];
+    snprintf(msg, sizeof(msg), "dmoe_kv_append: %s", what);
+    set_last_error(msg);
+    return st;
+  };
+  if (!a) return fail(DMOE_ERR_INVALID_ARG, "null pointer");
+  if (const dmoe_status st = kv_check("dmoe_kv_append", cache, batch, a->n_tokens, a->n_head)) return st;
+  const int hd = cache->head_dim, nk = cache->n_head_kv;
+  if (!is_float_type(a->qkv_type) || !is_float_type(a->q_type))
+    return fail(DMOE_ERR_UNSUPPORTED, "qkv and q_out are f32, f16 or bf16");
+  if (a->rotary_dim < 0 || a->rotary_dim > hd || a->rotary_dim % 16)
+    return fail(DMOE_ERR_UNSUPPORTED, "rotary_dim must be a multiple of 16 up to head_dim");
+  if (a->rotary_dim > 0 && !(a->rope_base > 0.0 && a->rope_base < INFINITY))
+    return fail(DMOE_ERR_INVALID_ARG, "rope_base must be positive");
+  if (a->qkv_stride < (int64_t)(a->n_head + 2 * nk) * hd || a->q_stride < (int64_t)a->n_head * hd)
+    return fail(DMOE_ERR_INVALID_ARG, "qkv_stride or q_stride is shorter than a row");
+  if (a->n_tokens == 0 || batch->n_seq == 0) return DMOE_OK;
+  if (!a->qkv || !a->q_out) return fail(DMOE_ERR_INVALID_ARG, "null pointer");
+  if ((reinterpret_cast<uintptr_t>(a->qkv) % size_of(a->qkv_type)) | (reinterpret_cast<uintptr_t>(a->q_out) % size_of(a->q_type)))
+    return fail(DMOE_ERR_INVALID_ARG, "qkv or q_out is not aligned to its elements");
+  if ((reinterpret_cast<uintptr_t>(a->q_norm) | reinterpret_cast<uintptr_t>(a->k_norm)) & 15u)
+    return fail(DMOE_ERR_INVALID_ARG, "q_norm and k_norm must be 16-byte aligned");
+
+  const NvtxRange nvtx_call("dmoe_kv_append");
+  AppendParams p{};
+  p.pg = kv_pages(cache);
+  p.b = kv_batch(batch, a->n_tokens);
+  p.qkv = a->qkv;
+  p.q_out = a->q_out;
+  p.q_norm = a->q_norm;
+  p.k_norm = a->k_norm;
+  p.qkv_stride = a->qkv_stride;
+  p.q_stride = a->q_stride;
+  p.qkv_type = a->qkv_type;
+  p.q_type = a->q_type;
+  p.n_head = a->n_head;
+  p.half = a->rotary_dim / 2;
+  p.eps = a->eps;
+  p.vec_in = aligned16(a->qkv, a->qkv_stride * size_of(a->qkv_type));
+  p.vec_out = aligned16(a->q_out, a->q_stride * size_of(a->q_type));
+  if (p.half > 0) {
+    // base^(-2i / r) as powers of one ratio: 63 products of 64 bits stay within 1e-14 of the power
+    const double ratio = pow(a->rope_base, -2.0 / a->rotary_dim);
+    double t = 0.15915494309189533577;  // 1 / 2 pi
+    for (int i = 0; i < p.half; ++i, t *= ratio) p.turns[i] = t;
+  }
+  const KvType kv = kv_type_of(cache->type);
+  // a sequence of f new rows touches at most f blocks, and at most f / 32 + 2
+  const int64_t units = std::min<int64_t>(a->n_tokens, a->n_tokens / kScaleBlock + 2ll * batch->n_seq);
+  const int held = kv == KV_E4M3 ? 2 * nk : 0;
+  p.flat_slots = a->n_head + 2 * nk - held;
+  p.flat_per_cta = p.flat_slots;
+  p.held_per_cta = std::max(1, held);
+  p.flat_groups = 1;
+  const int groups = p.flat_groups + (held ? 1 : 0);
+  const dim3 grid((unsigned)units, (unsigned)groups);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  void (*kernel)(AppendParams) = nullptr;
+  if (hd == 128)
+    kernel = kv == KV_BF16 ? kv_append_kernel<128, KV_BF16> : kv == KV_F16 ? kv_append_kernel<128, KV_F16> : kv_append_kernel<128, KV_E4M3>;
+  else
+    kernel = kv == KV_BF16 ? kv_append_kernel<64, KV_BF16> : kv == KV_F16 ? kv_append_kernel<64, KV_F16> : kv_append_kernel<64, KV_E4M3>;
+  kernel<<<grid, kThreads, 0, st>>>(p);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) {
+    char msg[256];
+    snprintf(msg, sizeof(msg), "launch failed: %s", cudaGetErrorString(e));
+    return fail(DMOE_ERR_CUDA, msg);
+  }
+  return DMOE_OK;
+}

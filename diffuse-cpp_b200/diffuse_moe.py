@@ -12,6 +12,7 @@ stream and `sync()` waits for it).
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from typing import Optional
@@ -22,7 +23,8 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libdiffuse_moe.so")
 
 # ggml_type ids (ggml.h)
-TYPE_F32, TYPE_F16, TYPE_Q8_0, TYPE_Q4_K = 0, 1, 8, 12
+TYPE_F32, TYPE_F16, TYPE_Q8_0, TYPE_Q4_K, TYPE_BF16 = 0, 1, 8, 12, 30
+TYPE_E4M3 = 1000  # 8-bit pages of a key/value cache (no ggml id)
 TYPE_NAMES = {TYPE_F32: "f32", TYPE_F16: "f16", TYPE_Q8_0: "q8_0", TYPE_Q4_K: "q4_K"}
 
 F_HOST_PTRS, F_ROUTE_ONLY, F_PROFILE, F_DETERMINISTIC = 1, 2, 4, 8
@@ -128,6 +130,65 @@ class ModelInfo(ctypes.Structure):
         return {name: getattr(self, name) for name, _ in self._fields_}
 
 
+class KVCacheDesc(ctypes.Structure):
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("err", ctypes.c_void_p),
+        ("n_pages", ctypes.c_int64),
+        ("n_head_kv", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("type", ctypes.c_int32),
+    ]
+
+
+class KVBatchDesc(ctypes.Structure):
+    _fields_ = [
+        ("page_table", ctypes.c_void_p),
+        ("q_start", ctypes.c_void_p),
+        ("kv_len", ctypes.c_void_p),
+        ("max_pages", ctypes.c_int64),
+        ("n_seq", ctypes.c_int32),
+        ("max_q_len", ctypes.c_int32),
+    ]
+
+
+class KVAppendArgs(ctypes.Structure):
+    _fields_ = [
+        ("qkv", ctypes.c_void_p),
+        ("q_out", ctypes.c_void_p),
+        ("q_norm", ctypes.c_void_p),
+        ("k_norm", ctypes.c_void_p),
+        ("n_tokens", ctypes.c_int64),
+        ("qkv_stride", ctypes.c_int64),
+        ("q_stride", ctypes.c_int64),
+        ("qkv_type", ctypes.c_int32),
+        ("q_type", ctypes.c_int32),
+        ("n_head", ctypes.c_int32),
+        ("rotary_dim", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("rope_base", ctypes.c_double),
+    ]
+
+
+class KVAttentionArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p),
+        ("n_tokens", ctypes.c_int64),
+        ("q_stride", ctypes.c_int64),
+        ("out_stride", ctypes.c_int64),
+        ("type", ctypes.c_int32),
+        ("n_head", ctypes.c_int32),
+        ("block_length", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+    ]
+
+
 class DmoeError(RuntimeError):
     def __init__(self, status: int, message: str):
         super().__init__(f"{STATUS_NAMES.get(status, status)}: {message}")
@@ -174,6 +235,12 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
     lib.dmoe_sample_step.argtypes = [P, ctypes.c_int64, ctypes.c_int64, P, ctypes.c_int32, ctypes.c_int32,
                                      ctypes.c_float, P, P, P, P]
     lib.dmoe_sample_step.restype = ctypes.c_int
+    lib.dmoe_kv_append.argtypes = [P, P, P, P]
+    lib.dmoe_kv_append.restype = ctypes.c_int
+    lib.dmoe_kv_attention_workspace.argtypes = [P, P, P]
+    lib.dmoe_kv_attention_workspace.restype = ctypes.c_size_t
+    lib.dmoe_kv_attention.argtypes = [P, P, P, P, ctypes.c_size_t, P]
+    lib.dmoe_kv_attention.restype = ctypes.c_int
     lib.dmoe_create_split.argtypes = [ctypes.POINTER(LayerDesc), ctypes.POINTER(DistCfg), P, ctypes.POINTER(P)]
     lib.dmoe_create_split.restype = ctypes.c_int
     lib.dmoe_model_load.argtypes = [ctypes.c_char_p, ctypes.POINTER(DistCfg), ctypes.POINTER(P)]
@@ -472,3 +539,161 @@ def sample_step(logits, seq, mask_id: int, n_transfer: int, threshold: float, to
     n_pos, n_vocab = int(logits.shape[0]), int(logits.shape[1])
     _check(load().dmoe_sample_step(_ptr(logits), n_pos, n_vocab, _ptr(seq), mask_id, n_transfer, threshold,
                                    _ptr(token), _ptr(prob), _ptr(n_committed), stream if stream else None))
+
+
+class KVBatch:
+    """The sequences of a paged-cache call (struct dmoe_kv_batch). torch int32 CUDA tensors, read by the
+    GPU when the call runs (their values may change between calls and graph replays): page_table
+    [n_seq, max_pages], q_start [n_seq + 1] (first row of each sequence in the row tensors), kv_len
+    [n_seq] (positions of each sequence, the call's rows included). max_q_len: an upper bound of
+    the rows of one sequence."""
+
+    def __init__(self, page_table, q_start, kv_len, max_q_len: int):
+        import torch
+
+        for name, t, dim in (("page_table", page_table, 2), ("q_start", q_start, 1), ("kv_len", kv_len, 1)):
+            if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.int32 or t.dim() != dim \
+                    or not t.is_contiguous() or t.device != page_table.device:
+                raise ValueError(f"KVBatch: {name} must be a contiguous {dim}-d int32 CUDA tensor, all on one device")
+        n = int(kv_len.shape[0])
+        if page_table.shape[0] != n or q_start.shape[0] != n + 1:
+            raise ValueError("KVBatch: page_table needs n_seq rows and q_start n_seq + 1 entries")
+        self.tensors = (page_table, q_start, kv_len)
+        self.device = page_table.device
+        self._desc = KVBatchDesc(_ptr(page_table), _ptr(q_start), _ptr(kv_len), int(page_table.shape[1]), n,
+                                 int(max_q_len))
+        self._ref = ctypes.addressof(self._desc)
+
+
+class PagedKV:
+    """Paged key/value cache of n_layer layers (struct dmoe_kv_cache per layer): n_pages pages of page_size
+    positions, shared by every sequence of a batch. kv_type "bf16", "f16", or "e4m3": 8 bits with a
+    power-of-two scale for every 32 positions of a head. k and v are [n_layer, n_pages, n_head_kv,
+    page_size, head_dim] (zeroed); in 8-bit pages k_scale and v_scale [n_layer, n_pages, n_head_kv,
+    page_size / 32] are torch.float8_e8m0fnu, and a value is code * scale.
+
+    append() writes a layer's new keys and values and returns the rotated queries; attend() is the
+    attention of queries over the pages. Both enqueue on the current torch stream (or `stream`) and can
+    be captured in CUDA graphs. check() reports what the kernels found wrong in a batch's tables."""
+
+    def __init__(self, n_pages: int, n_head_kv: int, head_dim: int, page_size: int = 64, kv_type: str = "e4m3",
+                 n_layer: int = 1, device="cuda"):
+        import torch
+
+        held = {"bf16": (TYPE_BF16, torch.bfloat16), "f16": (TYPE_F16, torch.float16),
+                "e4m3": (TYPE_E4M3, torch.float8_e4m3fn)}
+        if kv_type not in held:
+            raise ValueError(f"PagedKV: kv_type must be one of {sorted(held)}")
+        self.kv_type, self.n_layer, self.n_head_kv, self.head_dim = kv_type, n_layer, n_head_kv, head_dim
+        self.page_size, self.n_pages = page_size, n_pages
+        ctype, dtype = held[kv_type]
+        shape = (n_layer, n_pages, n_head_kv, page_size, head_dim)
+        self.k, self.v = (torch.zeros(shape, dtype=torch.uint8 if kv_type == "e4m3" else dtype, device=device).view(dtype)
+                          for _ in range(2))
+        self.k_scale = self.v_scale = None
+        if kv_type == "e4m3":
+            self.k_scale, self.v_scale = (torch.zeros(*shape[:3], max(1, page_size // 32), dtype=torch.uint8, device=device)
+                                          .view(torch.float8_e8m0fnu) for _ in range(2))
+        self.err = torch.zeros(1, dtype=torch.int32, device=device)
+        self.device = self.err.device
+        self._types = {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}
+        self._desc = []
+        for il in range(n_layer):
+            sc = (_ptr(self.k_scale[il]), _ptr(self.v_scale[il])) if kv_type == "e4m3" else (None, None)
+            self._desc.append(KVCacheDesc(_ptr(self.k[il]), _ptr(self.v[il]), *sc, _ptr(self.err), n_pages, n_head_kv,
+                                          head_dim, page_size, ctype))
+        self._ref = [ctypes.addressof(d) for d in self._desc]
+
+    def _rows(self, call: str, name: str, t, width: int, n: int = -1):
+        """Checks a row tensor ([n, width] elements, rows any distance apart); its type id and row stride."""
+        kind = self._types.get(t.dtype)
+        if kind is None or t.device != self.device:
+            raise ValueError(f"{call}: {name} must be a float32, float16 or bfloat16 tensor on {self.device}")
+        shape = t.shape
+        dense = len(shape) == 2 and shape[1] == width and (t.stride(1) == 1 or width == 1)
+        if not dense and len(shape) == 3:
+            dense = shape[1] * shape[2] == width and t.stride(2) == 1 and t.stride(1) == shape[2]
+        if not dense or (n >= 0 and shape[0] != n):
+            raise ValueError(f"{call}: {name} must hold {'n' if n < 0 else n} rows of {width} consecutive elements")
+        return kind, t.stride(0) if shape[0] > 1 else max(width, t.stride(0))
+
+    def _launch(self, batch: KVBatch, stream, fn):
+        import torch
+
+        if batch.device != self.device:
+            raise ValueError("PagedKV: the batch and the cache are on different devices")
+        if stream is None:
+            stream = torch.cuda.current_stream(self.device).cuda_stream
+        if torch.cuda.current_device() != self.device.index:
+            with torch.cuda.device(self.device):
+                return fn(stream)
+        return fn(stream)
+
+    def append(self, layer: int, qkv, batch: KVBatch, n_head: int, q_norm=None, k_norm=None, eps: float = 1e-6,
+               rotary_dim: int = 0, rope_base: float = 10000.0, q_type=None, q_out=None, stream: Optional[int] = None):
+        """dmoe_kv_append: qkv [n, (n_head + 2 n_head_kv) head_dim] (float32, float16 or bfloat16) -> the rotated
+        queries [n, n_head, head_dim] (q_out, or a new tensor of q_type, default qkv's). q_norm and k_norm:
+        [head_dim] float32, or None for no normalisation. Rows that belong to no sequence are not
+        written: in a new tensor they are uninitialised."""
+        import torch
+
+        n = int(qkv.shape[0])
+        kind, stride = self._rows("append", "qkv", qkv, (n_head + 2 * self.n_head_kv) * self.head_dim)
+        if q_out is None:
+            q_out = torch.empty((n, n_head, self.head_dim), dtype=q_type or qkv.dtype, device=self.device)
+        q_kind, q_stride = self._rows("append", "q_out", q_out, n_head * self.head_dim, n)
+        for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
+            if w is not None and (w.dtype != torch.float32 or w.device != self.device or w.shape != (self.head_dim,)
+                                  or not w.is_contiguous()):
+                raise ValueError(f"append: {name} must be a contiguous float32 [head_dim] tensor on {self.device}")
+        args = KVAppendArgs(qkv.data_ptr(), q_out.data_ptr(), _ptr(q_norm) or None, _ptr(k_norm) or None, n, stride,
+                            q_stride, kind, q_kind, n_head, rotary_dim, eps, rope_base)
+        _check(self._launch(batch, stream, lambda st: load().dmoe_kv_append(
+            self._ref[layer], batch._ref, ctypes.addressof(args), st or None)))
+        return q_out
+
+    def attend(self, layer: int, q, batch: KVBatch, block_length: int = 1, scale: Optional[float] = None, out=None,
+               lse=None, stream: Optional[int] = None):
+        """dmoe_kv_attention: q [n, n_head, head_dim] (float16 or bfloat16) -> the attention's output, of q's shape
+        and type. A row at position p sees the positions j < kv_len with j // block_length <= p // block_length.
+        scale: default head_dim ** -0.5. lse: [n, n_head] float32 for the logarithms of the softmax sums, or
+        None. Rows that belong to no sequence are not written."""
+        import torch
+
+        if q.dim() != 3 or q.shape[2] != self.head_dim:
+            raise ValueError("attend: q must be [n, n_head, head_dim]")
+        n, n_head = int(q.shape[0]), int(q.shape[1])
+        kind, stride = self._rows("attend", "q", q, n_head * self.head_dim)
+        if out is None:
+            out = torch.empty((n, n_head, self.head_dim), dtype=q.dtype, device=self.device)
+        o_kind, o_stride = self._rows("attend", "out", out, n_head * self.head_dim, n)
+        if o_kind != kind:
+            raise ValueError("attend: out must have q's type")
+        if lse is not None and (lse.dtype != torch.float32 or lse.device != self.device or lse.shape != (n, n_head)
+                                or not lse.is_contiguous()):
+            raise ValueError(f"attend: lse must be a contiguous float32 [n, n_head] tensor on {self.device}")
+        args = KVAttentionArgs(q.data_ptr(), out.data_ptr(), _ptr(lse) or None, n, stride, o_stride, kind, n_head,
+                               block_length, scale if scale is not None else self.head_dim ** -0.5)
+        lib, ref = load(), ctypes.addressof(args)
+
+        def call(st):
+            size = lib.dmoe_kv_attention_workspace(self._ref[layer], batch._ref, ref)
+            ws = None
+            if size:  # of the launching stream's pool: calls on different streams and graphs have their own
+                with torch.cuda.stream(torch.cuda.ExternalStream(st, device=self.device)) if stream is not None \
+                        else contextlib.nullcontext():
+                    ws = torch.empty(size, dtype=torch.uint8, device=self.device)
+            return lib.dmoe_kv_attention(self._ref[layer], batch._ref, ref, _ptr(ws) or None, size, st or None)
+
+        _check(self._launch(batch, stream, call))
+        return out
+
+    def check(self) -> None:
+        """Waits for the device and raises if a kernel met a page number or a batch entry out of its bounds
+        since the last check (such entries are skipped, see include/diffuse_moe.h)."""
+        bits = int(self.err.item())
+        if bits:
+            self.err.zero_()
+            what = [w for b, w in ((1, "page number out of range"), (2, "invalid q_start / kv_len / max_q_len"),
+                                   (4, "a device-side wait timed out")) if bits & b]
+            raise DmoeError(6 if bits & 4 else 1, "paged cache: " + ", ".join(what))

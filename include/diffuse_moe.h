@@ -45,7 +45,9 @@ enum {
   DMOE_TYPE_F32 = 0,
   DMOE_TYPE_F16 = 1,
   DMOE_TYPE_Q8_0 = 8,
-  DMOE_TYPE_Q4_K = 12
+  DMOE_TYPE_Q4_K = 12,
+  DMOE_TYPE_BF16 = 30,
+  DMOE_TYPE_E4M3 = 1000 /* 8-bit pages of a key/value cache (no ggml id): see dmoe_kv_cache */
 };
 
 /* One MoE layer: the tensors of struct diffuse_moe_layer (src/diffuse-common.h:72-82) and the
@@ -289,6 +291,110 @@ dmoe_status dmoe_route_static(const float* x, int64_t n_tokens, int64_t n_embd, 
 dmoe_status dmoe_sample_step(const float* logits, int64_t n_pos, int64_t n_vocab, int32_t* seq, int32_t mask_id,
                              int32_t n_transfer, float threshold, int32_t* token, float* prob,
                              int32_t* n_committed, void* stream);
+
+/* ---- Paged key/value cache: append with rotation, and attention over its pages.
+ * The reference recomputes every position's keys and values at every denoising step
+ * (src/diffuse-moe-graph.cpp:126-175 inside the loop of src/diffuse-sampler.cpp:144-258) and has no
+ * cache. Here a batch of sequences of unequal length shares one pool of pages, and two calls per
+ * layer replace :142-175: dmoe_kv_append (split of the fused QKV, QK norm :145-150, RoPE :155-161,
+ * the write into the pages) and dmoe_kv_attention (:163-175 under the block-causal mask :38-52). */
+
+/* One layer's pages, all DEVICE memory of the caller, laid out [n_pages][n_head_kv][page_size]
+ * [head_dim]. type: DMOE_TYPE_BF16, DMOE_TYPE_F16, or DMOE_TYPE_E4M3: 8-bit values (4 exponent and 3
+ * mantissa bits, no infinity) with one scale for every DMOE_KV_SCALE_BLOCK positions of a head,
+ * [n_pages][n_head_kv][page_size / DMOE_KV_SCALE_BLOCK] bytes b standing for 2^(b - 127): the
+ * smallest 2^e, -60 <= e <= 120, with max |x| <= 448 * 2^e over the block's positions. A value that
+ * is not finite is held as NaN. page_size is a multiple of 32 (so a scale block lies in one page),
+ * head_dim 64 or 128; k and v are 16-byte aligned.
+ * err (optional, one word): device-side findings are OR-ed into it (DMOE_KV_ERR_*); the call
+ * itself cannot report them, since the tables are device memory. The caller zeroes and reads it. */
+#define DMOE_KV_SCALE_BLOCK 32
+typedef struct dmoe_kv_cache {
+  void* k;
+  void* v;
+  uint8_t* k_scale;  /* DMOE_TYPE_E4M3 only */
+  uint8_t* v_scale;
+  uint32_t* err;
+  int64_t n_pages;
+  int32_t n_head_kv;
+  int32_t head_dim;
+  int32_t page_size;
+  int32_t type;
+} dmoe_kv_cache;
+
+#define DMOE_KV_ERR_PAGE 1u    /* a page number outside [0, n_pages): such a position is not written;
+                                  attention then reads page 0 in its place */
+#define DMOE_KV_ERR_BATCH 2u   /* q_start not ascending within [0, n_tokens], kv_len negative or over
+                                  max_pages pages, or more than max_q_len queries: the sequence is
+                                  skipped (its rows are left as they were) */
+#define DMOE_KV_ERR_TIMEOUT 4u /* a bounded device-side wait expired: the outputs are not complete */
+
+/* The sequences of a call. Sequence s owns the rows [q_start[s], q_start[s + 1]) of the row tensors;
+ * kv_len[s] counts its positions with those rows included, so that its row i stands at position
+ * kv_len[s] - q_len + i. Rows at negative positions (a batch padded on the left) are padding: they
+ * enter no cache, and their outputs are zero. Rows behind q_start[n_seq] are not touched.
+ * Position p lies in page page_table[s][p / page_size] at p % page_size; entries past kv_len are not
+ * read. Pages that a call writes must belong to one sequence; pages that are only read may be
+ * shared. max_q_len is an upper bound of the rows of a sequence. */
+typedef struct dmoe_kv_batch {
+  const int32_t* page_table; /* DEVICE, [n_seq][max_pages] */
+  const int32_t* q_start;    /* DEVICE, [n_seq + 1] */
+  const int32_t* kv_len;     /* DEVICE, [n_seq] */
+  int64_t max_pages;
+  int32_t n_seq;
+  int32_t max_q_len;
+} dmoe_kv_batch;
+
+/* Splits every row of qkv into [n_head query; n_head_kv key; n_head_kv value] heads; normalises query
+ * and key heads (x / sqrt(mean x^2 + eps) * weight; NULL weight: not normalised); rotates their first
+ * rotary_dim dims as two halves by theta_i = position * rope_base^(-2 i / rotary_dim); writes keys and
+ * values into the pages and the queries to q_out. Positions from the row's own on are overwritten or
+ * void: in 8-bit pages the last scale blocks are formed from what the block keeps and the new
+ * rows (kept values move to a new scale exactly, unless they fall below 2^-6 of it). qkv and q_out:
+ * DMOE_TYPE_F32, F16 or BF16, rows of qkv_stride / q_stride elements. rotary_dim: a multiple of 16 up
+ * to head_dim, 0 for no rotation. Enqueued on `stream` (NULL: the default stream). */
+typedef struct dmoe_kv_append_args {
+  const void* qkv;
+  void* q_out;          /* [n_tokens][n_head][head_dim] */
+  const float* q_norm;  /* [head_dim] or NULL */
+  const float* k_norm;
+  int64_t n_tokens;
+  int64_t qkv_stride;   /* elements between rows */
+  int64_t q_stride;
+  int32_t qkv_type;
+  int32_t q_type;
+  int32_t n_head;
+  int32_t rotary_dim;
+  float eps;
+  double rope_base;
+} dmoe_kv_append_args;
+dmoe_status dmoe_kv_append(const dmoe_kv_cache* cache, const dmoe_kv_batch* batch, const dmoe_kv_append_args* args,
+                           void* stream);
+
+/* out = softmax(scale q k^T) v over the pages: row at position p sees positions j < kv_len with
+ * j / block_length <= p / block_length (1: causal; the model's block length: block-causal). Query head
+ * h reads key/value head h / (n_head / n_head_kv). lse (optional) [n_tokens][n_head]: the natural
+ * logarithm of each softmax's sum, -inf for rows that see nothing (their output is zero). q and out:
+ * DMOE_TYPE_F16 or BF16, of one type; rows of q_stride / out_stride elements. workspace: DEVICE,
+ * 16-byte aligned, dmoe_kv_attention_workspace() bytes, uninitialised; calls that may overlap need one
+ * each. A value that is not finite reaches only the rows that see its position. */
+typedef struct dmoe_kv_attention_args {
+  const void* q;        /* [n_tokens][n_head][head_dim] */
+  void* out;            /* [n_tokens][n_head][head_dim] */
+  float* lse;
+  int64_t n_tokens;
+  int64_t q_stride;     /* elements between rows */
+  int64_t out_stride;
+  int32_t type;
+  int32_t n_head;
+  int32_t block_length;
+  float scale;
+} dmoe_kv_attention_args;
+size_t dmoe_kv_attention_workspace(const dmoe_kv_cache* cache, const dmoe_kv_batch* batch,
+                                   const dmoe_kv_attention_args* args);
+dmoe_status dmoe_kv_attention(const dmoe_kv_cache* cache, const dmoe_kv_batch* batch,
+                              const dmoe_kv_attention_args* args, void* workspace, size_t workspace_bytes,
+                              void* stream);
 
 #ifdef __cplusplus
 }
