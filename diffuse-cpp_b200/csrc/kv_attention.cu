@@ -43,8 +43,9 @@ struct AttnParams {
   int n_head, group;
   int block_length;
   int n_qt;          // row tiles a sequence can have (max_q_len)
-  int vec_q;         // q rows allow 8-byte loads
+  int vec_q, vec_q16, vec_out16;  // q rows allow 8-byte, 16-byte loads; out rows 16-byte stores
   float scale_log2;  // scale * log2(e)
+  uint32_t* wait_err;  // word that bounded waits report to
   float* part;       // partial triples, slot = 2 * CTA + (the item begins in this CTA)
   int4* desc;        // [CTA] {item, head, last CTA, 1} of the item this CTA begins and does not end
 };
@@ -591,44 +592,665 @@ __global__ void __launch_bounds__(256, 1) kv_rows_kernel(const __grid_constant__
   pdl_trigger();
 }
 
+// ---------------------------------------------------------------------------------------------
+// Many rows (denoising blocks, prompts): tensor-core tiles of 2 x 128 rows by 128 positions.
+//
+// One persistent CTA per SM. Warps 0-3 and 4-7: softmax of the two 128-row halves, a thread a row; warps
+// 8-11: keys and values from the pages into shared memory, as 16-bit operands in the 128-byte swizzle;
+// warp 12 issues the products. TMEM: two score tiles (f32, 128 columns each; a half's weights
+// overwrite its scores as the 16-bit A operand of the second product) and two outputs. The products of one
+// half run while the other half's softmax does. The running maximum that weights refer to follows
+// the true one only when that is 2^8 ahead (f16 holds the weights up to then), so an output is
+// rescaled in TMEM only then.
+// Bound by the tensor cores together with the exponentials: a 128-cube of products takes 512 cycles, the
+// 128 x 128 exponentials between two of them 1024 of one SM's 16 a cycle, shared by two products.
+// ---------------------------------------------------------------------------------------------
+template <int HD, int KV>
+struct TileCfg {
+  static constexpr int R = 256, TILE = 128;
+  static constexpr int ES = KV == KV_E4M3 ? 1 : 2;
+  static constexpr int kThreads = 416, kLoaders = 128;
+  static constexpr int kPlane = 128 * 128;             // 64 elements of 128 rows
+  static constexpr int kOperand = HD / 64 * kPlane;    // bytes of a 128-row operand
+  static constexpr int kStages = 2;
+  static constexpr size_t kSmem = 1024 + (2 + 2 * kStages) * (size_t)kOperand;
+  static constexpr int kPart = R * (HD + 2);
+};
+
+struct TileBars {
+  uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], read[4], reset, done;
+};
+
+// mbar_wait by a whole warp, with one answer: after a timeout no lane goes on alone
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, uint32_t* err, uint32_t bit) {
+  const bool ok = mbar_wait(bar, parity, err, bit);
+  return __all_sync(0xffffffffu, ok);
+}
+
+// walks a CTA's run, item by item: what every warp role does on its own
+template <int R, int TILE>
+struct Walk {
+  const AttnParams& p;
+  Run run;
+  Item it{};
+  int u, head, seg = 0;
+  int64_t tile0, tile1, at;
+  __device__ Walk(const AttnParams& p_, const Run& r) : p(p_), run(r), u(r.u), head(r.head), tile0(r.tile), tile1(0), at(r.first) {
+    if (run.left > 0) {
+      it = item_of<R, TILE>(p, u);
+      tile1 = min((int64_t)it.tiles, tile0 + run.left);
+    }
+  }
+  __device__ bool more() const { return run.left > 0; }
+  __device__ void next() {
+    run.left -= tile1 - tile0;
+    at += tile1 - tile0;
+    tile0 = 0;
+    ++seg;
+    if (run.left <= 0) return;
+    if (++head == p.pg.n_head_kv) {
+      head = 0;
+      do it = item_of<R, TILE>(p, ++u);
+      while (it.tiles == 0);
+    }
+    tile1 = min((int64_t)it.tiles, run.left);
+  }
+};
+
+template <int HD, int KV>
+__global__ void __launch_bounds__(416, 1) kv_tile_kernel(const __grid_constant__ AttnParams p) {
+  using C = TileCfg<HD, KV>;
+  constexpr bool kBf = KV == KV_BF16;
+  constexpr int R = C::R, TILE = C::TILE, ES = C::ES;
+  constexpr uint32_t kIdescS = idesc_16b_f32(128, 128, kBf, false), kIdescO = idesc_16b_f32(128, HD, kBf, true);
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ TileBars bar;
+  __shared__ uint32_t tmem_base_s;
+  __shared__ int64_t sums[C::kThreads / 32];
+  __shared__ Run found;
+  __shared__ int not_finite_from[4][HD];  // [item of the run & 3][d]: first position whose value is not finite
+  __shared__ int any_not_finite[4];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* q_s = smem;                                 // [half] operands
+  uint8_t* k_s = q_s + 2 * C::kOperand;                // [stage]
+  uint8_t* v_s = k_s + C::kStages * C::kOperand;       // [stage]
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+
+  if (warp == 12) {
+    tmem_alloc(&tmem_base_s, 512);
+    tmem_relinquish();
+  }
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bar.q_full[i], 128);
+      mbar_init(&bar.k_full[i], C::kLoaders);
+      mbar_init(&bar.k_empty[i], 1);
+      mbar_init(&bar.v_full[i], C::kLoaders);
+      mbar_init(&bar.v_empty[i], 1);
+      mbar_init(&bar.s_full[i], 1);
+      mbar_init(&bar.p_full[i], 128);
+      mbar_init(&bar.o_full[i], 1);
+    }
+    for (int i = 0; i < 4; ++i) mbar_init(&bar.read[i], 256);
+    mbar_init(&bar.reset, C::kLoaders);
+    mbar_init(&bar.done, 1);
+    fence_mbar_init();
+  }
+  if (tid < 4) any_not_finite[tid] = 0;
+  tc_fence_before();
+  const Run run = find_run<R, TILE, C::kThreads>(p, sums, &found);  // ends with a barrier of the CTA
+  tc_fence_after();
+  const uint32_t tmem = tmem_base_s;
+  uint32_t* err = p.wait_err;
+  constexpr uint32_t kTimeout = DMOE_KV_ERR_TIMEOUT;
+  Walk<R, TILE> w(p, run);
+
+  if (warp == 12) {
+    // ---- products
+    uint32_t kv_n = 0;           // tiles whose keys were used
+    uint32_t ph_q[2] = {0, 0}, ph_p[2] = {0, 0};
+    bool ok = true;
+    const uint32_t k_addr = smem_u32(k_s), v_addr = smem_u32(v_s), q_addr = smem_u32(q_s);
+    auto scores = [&](int half, int stage) {
+      if (elect_one()) {
+        const uint32_t qa = q_addr + half * C::kOperand, ka = k_addr + stage * C::kOperand;
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k) {
+          const uint32_t off = (k / 4) * C::kPlane + (k % 4) * 32;
+          mma_f16_ss(tmem + half * 128, sdesc_sw128(qa + off, 1024), sdesc_sw128(ka + off, 1024), kIdescS, k > 0);
+        }
+        mma_commit(&bar.s_full[half]);
+      }
+      __syncwarp();
+    };
+    auto outputs = [&](int half, int stage, bool first) {
+      if (elect_one()) {
+        const uint32_t va = v_addr + stage * C::kOperand;
+#pragma unroll
+        for (int k = 0; k < TILE / 16; ++k)
+          mma_f16_ts(tmem + 256 + half * 128, tmem + half * 128 + 8 * k, sdesc_sw128_mn(va + 2048 * k, C::kPlane), kIdescO,
+                     !(first && k == 0));
+      }
+      __syncwarp();
+    };
+    auto commit = [&](uint64_t* b) {
+      if (elect_one()) mma_commit(b);
+      __syncwarp();
+    };
+    for (; ok && w.more(); w.next()) {
+      const int halves = w.it.rows > 128 ? 2 : 1;
+      const int n = (int)(w.tile1 - w.tile0);
+      for (int h = 0; ok && h < halves; ++h) {
+        ok = warp_wait(&bar.q_full[h], ph_q[h], err, kTimeout);
+        ph_q[h] ^= 1;
+      }
+      if (ok) ok = warp_wait(&bar.k_full[kv_n & 1], (kv_n >> 1) & 1, err, kTimeout);
+      if (!ok) break;
+      tc_fence_after();
+      for (int h = 0; h < halves; ++h) scores(h, kv_n & 1);
+      commit(&bar.k_empty[kv_n & 1]);
+      for (int j = 0; ok && j < n; ++j, ++kv_n) {
+        const int stage = kv_n & 1, next = (kv_n + 1) & 1;
+        ok = warp_wait(&bar.v_full[stage], (kv_n >> 1) & 1, err, kTimeout);
+        for (int h = 0; ok && h < halves; ++h) {
+          ok = warp_wait(&bar.p_full[h], ph_p[h], err, kTimeout);
+          if (!ok) break;
+          ph_p[h] ^= 1;
+          tc_fence_after();
+          outputs(h, stage, j == 0);
+          if (h == halves - 1) commit(&bar.v_empty[stage]);
+          if (j + 1 < n) {
+            if (h == 0) ok = warp_wait(&bar.k_full[next], ((kv_n + 1) >> 1) & 1, err, kTimeout);
+            if (!ok) break;
+            tc_fence_after();
+            scores(h, next);
+            if (h == halves - 1) commit(&bar.k_empty[next]);
+          } else {
+            commit(&bar.o_full[h]);
+          }
+        }
+      }
+    }
+    commit(&bar.done);  // every product that was issued has ended before TMEM is freed
+    warp_wait(&bar.done, 0, err, kTimeout);
+  } else if (warp >= 8) {
+    // ---- keys and values
+    const int lt = tid - 256;
+    constexpr int LPR = HD * ES / 16;             // lanes a row, 16 bytes each
+    constexpr int RPI = C::kLoaders / LPR;        // rows an instruction of all loaders covers
+    constexpr int N = TILE / RPI;                 // 16-byte pieces a thread loads of a tile
+    const int c = lt % LPR, r0 = lt / LPR;
+    uint32_t kv_n = 0;
+    bool ok = true;
+    int pages[4];  // of the tile's 32-position groups
+    auto get_pages = [&](const Item& it, int64_t tile, int lim) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int64_t pos = tile * TILE + 32 * i;
+        pages[i] = 0;
+        if (pos < lim) {
+          pages[i] = p.b.table[it.seq * p.b.max_pages + pos / p.pg.page_size];
+          if (pages[i] < 0 || pages[i] >= p.pg.n_pages) {
+            kv_report(p.pg.err, DMOE_KV_ERR_PAGE);
+            pages[i] = 0;
+          }
+        }
+      }
+    };
+    // byte offset of row r of the tile, at this thread's piece
+    auto source = [&](int head, int64_t tile, int r) {
+      const int off = (int)((tile * TILE + (r & ~31)) % p.pg.page_size) + (r & 31);
+      return kv_row(p.pg, pages[r >> 5], head, off) * (HD * ES) + 16 * c;
+    };
+    // positions that only some rows see, and values that are not finite there: their products with a zero
+    // weight would reach the others. They are set to zero, and their element marked for the rows that see them
+    auto mark = [&](int seg, int pos, int d) {
+      atomicMin(&not_finite_from[seg & 3][d], pos);
+      any_not_finite[seg & 3] = 1;
+    };
+    auto reset_marks = [&](int seg) {
+      // once both halves have read the buffer's last use, four items back
+      if (!warp_wait(&bar.read[seg & 3], ((seg >> 2) & 1) ^ 1, err, kTimeout)) return false;
+      if (lt < HD) not_finite_from[seg & 3][lt] = INT32_MAX;
+      if (lt == 0) any_not_finite[seg & 3] = 0;
+      mbar_arrive(&bar.reset);
+      return warp_wait(&bar.reset, seg & 1, err, kTimeout);
+    };
+    if constexpr (KV == KV_E4M3) {
+      uint4 kr[N], vr[N];
+      auto fetch = [&](uint4 (&x)[N], const void* base, int head, int64_t tile, int lim) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const int r = r0 + i * RPI;
+          x[i] = make_uint4(0, 0, 0, 0);
+          if (tile * TILE + r < lim) x[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(base) + source(head, tile, r)));
+        }
+      };
+      auto put = [&](const uint4 (&x)[N], uint8_t* dst) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const int r = r0 + i * RPI;
+          const uint32_t v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+          uint32_t h[8];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) h[2 * e] = e4m3_pair<0>(v[e]), h[2 * e + 1] = e4m3_pair<1>(v[e]);
+          const uint4 a = make_uint4(h[0], h[1], h[2], h[3]), b = make_uint4(h[4], h[5], h[6], h[7]);
+          uint8_t* row = dst + (c / 4) * C::kPlane + r * 128;
+          const int first = (c / 4) & 1;  // lanes of the two planes take turns: no bank twice
+          const int ca = (2 * (c % 4)) ^ (r & 7), cb = (2 * (c % 4) + 1) ^ (r & 7);
+          *reinterpret_cast<uint4*>(row + 16 * (first ? cb : ca)) = first ? b : a;
+          *reinterpret_cast<uint4*>(row + 16 * (first ? ca : cb)) = first ? a : b;
+        }
+      };
+      if (w.more()) {
+        const int lim = row_limit(p, w.it.q, w.it.row_lo + w.it.rows - 1);
+        get_pages(w.it, w.tile0, lim);
+        fetch(kr, p.pg.k, w.head, w.tile0, lim);
+        fetch(vr, p.pg.v, w.head, w.tile0, lim);
+      }
+      while (ok && w.more()) {
+        const int lim_min = row_limit(p, w.it.q, w.it.row_lo);
+        const int lim_max = row_limit(p, w.it.q, w.it.row_lo + w.it.rows - 1);
+        const int seg = w.seg, head = w.head;
+        const Item it = w.it;
+        const int64_t t0 = w.tile0, t1 = w.tile1;
+        w.next();
+        for (int64_t t = t0; t < t1; ++t, ++kv_n) {
+          const int stage = kv_n & 1;
+          const uint32_t ph = ((kv_n >> 1) & 1) ^ 1;
+          ok = warp_wait(&bar.k_empty[stage], ph, err, kTimeout);
+          if (!ok) break;
+          put(kr, k_s + stage * C::kOperand);
+          fence_proxy_async_smem();
+          mbar_arrive(&bar.k_full[stage]);
+          // the next tile of this item or of the next one
+          const bool same = t + 1 < t1, more = same || w.more();
+          const Item& ni = same ? it : w.it;
+          const int nh = same ? head : w.head;
+          const int64_t nt = same ? t + 1 : w.tile0;
+          const int nl = same ? lim_max : more ? row_limit(p, w.it.q, w.it.row_lo + w.it.rows - 1) : 0;
+          if (more) {
+            get_pages(ni, nt, nl);
+            fetch(kr, p.pg.k, nh, nt, nl);
+          }
+          ok = warp_wait(&bar.v_empty[stage], ph, err, kTimeout);
+          if (!ok) break;
+          if (t == t0 && !reset_marks(seg)) {
+            ok = false;
+            break;
+          }
+          if (lim_min < lim_max && (t + 1) * TILE > lim_min) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+              const int pos = (int)(t * TILE) + r0 + i * RPI;
+              uint32_t v[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const uint32_t bad = __vcmpeq4(v[e] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+                if (bad && pos >= lim_min) {
+                  for (int b = 0; b < 4; ++b)
+                    if ((bad >> (8 * b)) & 1u) mark(seg, pos, 16 * c + 4 * e + b);
+                  v[e] &= ~bad;
+                }
+              }
+              vr[i] = make_uint4(v[0], v[1], v[2], v[3]);
+            }
+          }
+          put(vr, v_s + stage * C::kOperand);
+          fence_proxy_async_smem();
+          mbar_arrive(&bar.v_full[stage]);
+          if (more) fetch(vr, p.pg.v, nh, nt, nl);
+        }
+      }
+    } else {
+      // 16-bit pages need no conversion: asynchronous copies, the next tile's keys ahead of this one's arrival
+      auto issue = [&](const void* base, uint8_t* dst, int head, int64_t tile, int lim) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const int r = r0 + i * RPI;
+          const bool in = tile * TILE + r < lim;
+          const uint8_t* src = static_cast<const uint8_t*>(base) + (in ? source(head, tile, r) : 0);
+          const uint32_t to = smem_u32(dst) + (c / 8) * C::kPlane + r * 128 + 16 * ((c % 8) ^ (r & 7));
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(src), "r"(in ? 16 : 0) : "memory");
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      };
+      if (w.more()) {
+        const int lim = row_limit(p, w.it.q, w.it.row_lo + w.it.rows - 1);
+        get_pages(w.it, w.tile0, lim);
+        issue(p.pg.k, k_s, w.head, w.tile0, lim);  // the ring is empty
+        issue(p.pg.v, v_s, w.head, w.tile0, lim);
+      }
+      while (ok && w.more()) {
+        const int lim_min = row_limit(p, w.it.q, w.it.row_lo);
+        const int lim_max = row_limit(p, w.it.q, w.it.row_lo + w.it.rows - 1);
+        const int seg = w.seg, head = w.head;
+        const Item it = w.it;
+        const int64_t t0 = w.tile0, t1 = w.tile1;
+        w.next();
+        for (int64_t t = t0; t < t1; ++t, ++kv_n) {
+          const int stage = kv_n & 1, next = (kv_n + 1) & 1;
+          const uint32_t ph = (((kv_n + 1) >> 1) & 1) ^ 1;
+          const bool same = t + 1 < t1, more = same || w.more();
+          const Item& ni = same ? it : w.it;
+          const int nh = same ? head : w.head;
+          const int64_t nt = same ? t + 1 : w.tile0;
+          const int nl = same ? lim_max : more ? row_limit(p, w.it.q, w.it.row_lo + w.it.rows - 1) : 0;
+          if (more) {
+            get_pages(ni, nt, nl);
+            ok = warp_wait(&bar.k_empty[next], ph, err, kTimeout);
+            if (!ok) break;
+            issue(p.pg.k, k_s + next * C::kOperand, nh, nt, nl);
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+          } else {
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+          }
+          if (t == t0 && !reset_marks(seg)) {
+            ok = false;
+            break;
+          }
+          if (lim_min < lim_max && (t + 1) * TILE > lim_min) {
+#pragma unroll 1
+            for (int i = 0; i < N; ++i) {
+              const int r = r0 + i * RPI, pos = (int)(t * TILE) + r;
+              uint4* at = reinterpret_cast<uint4*>(v_s + stage * C::kOperand + (c / 8) * C::kPlane + r * 128 + 16 * ((c % 8) ^ (r & 7)));
+              const uint4 x = *at;  // this thread's own copy
+              uint32_t v[4] = {x.x, x.y, x.z, x.w};
+              bool found_bad = false;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                constexpr uint32_t kExp = kBf ? 0x7f807f80u : 0x7c007c00u;
+                const uint32_t bad = __vcmpeq2(v[e] & kExp, kExp);
+                if (bad && pos >= lim_min) {
+                  for (int b = 0; b < 2; ++b)
+                    if ((bad >> (16 * b)) & 1u) mark(seg, pos, 8 * c + 2 * e + b);
+                  v[e] &= ~bad;
+                  found_bad = true;
+                }
+              }
+              if (found_bad) *at = make_uint4(v[0], v[1], v[2], v[3]);
+            }
+          }
+          fence_proxy_async_smem();
+          mbar_arrive(&bar.k_full[stage]);
+          mbar_arrive(&bar.v_full[stage]);
+          if (more) {
+            ok = warp_wait(&bar.v_empty[next], ph, err, kTimeout);
+            if (!ok) break;
+            issue(p.pg.v, v_s + next * C::kOperand, nh, nt, nl);
+          }
+        }
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+    }
+  } else {
+    // ---- softmax of one half
+    const int half = warp >> 2, quarter = warp & 3;
+    const int my = half * 128 + quarter * 32 + lane;  // row of the item
+    const uint32_t s_addr = tmem_addr(tmem, quarter * 32, half * 128), o_addr = tmem_addr(tmem, quarter * 32, 256 + half * 128);
+    uint32_t ph_s = 0, ph_o = 0;
+    bool ok = true;
+    int4 begun = make_int4(0, 0, 0, 0);
+    for (; ok && w.more(); w.next()) {
+      const Item& it = w.it;
+      const bool whole = w.tile0 == 0 && w.tile1 == it.tiles;
+      if (!whole && w.tile0 == 0) begun = make_int4(w.u, w.head, (int)((w.at + it.tiles - 1) / run.chunk), 1);
+      if (half * 128 >= it.rows) {
+        mbar_arrive(&bar.read[w.seg & 3]);
+        continue;
+      }
+      const bool live = my < it.rows;
+      const int row = it.row_lo + my;
+      // the row's queries into the operand, scaled into [-1, 1] for f16 products
+      float factor = p.scale_log2;
+      {
+        uint32_t x[HD / 2];
+        const int64_t at = (int64_t)(it.q.row0 + row / p.group) * p.q_stride + (int64_t)(w.head * p.group + row % p.group) * HD;
+#pragma unroll
+        for (int i = 0; i < HD / 8; ++i) {
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (live) {
+            if (p.vec_q16) {
+              v = __ldg(reinterpret_cast<const uint4*>(p.q + at) + i);
+            } else {
+              const uint16_t* s = p.q + at + 8 * i;
+              v = make_uint4(s[0] | (uint32_t)s[1] << 16, s[2] | (uint32_t)s[3] << 16, s[4] | (uint32_t)s[5] << 16,
+                             s[6] | (uint32_t)s[7] << 16);
+            }
+          }
+          x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
+        }
+        auto value = [&](uint32_t v) {
+          if (p.is_bf16) return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+          return __half22float2(*reinterpret_cast<const __half2*>(&v));
+        };
+        if (!(kBf && p.is_bf16)) {
+          float inv = 1.f;
+          if (!kBf) {
+            float amax = 0.f;
+#pragma unroll
+            for (int i = 0; i < HD / 2; ++i) {
+              const float2 f = value(x[i]);
+              amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+            }
+            const int e = min(max((int)(__float_as_uint(amax) >> 23) - 126, -100), 100);
+            inv = pow2i(-e);
+            factor *= pow2i(e);
+          }
+#pragma unroll
+          for (int i = 0; i < HD / 2; ++i) {
+            const float2 f = value(x[i]);
+            x[i] = pack2<kBf>(f.x * inv, f.y * inv);
+          }
+        }
+        const int r = quarter * 32 + lane;
+        uint8_t* dst = q_s + half * C::kOperand + r * 128;
+#pragma unroll
+        for (int i = 0; i < HD / 8; ++i)
+          *reinterpret_cast<uint4*>(dst + (i / 8) * C::kPlane + 16 * ((i % 8) ^ (r & 7))) =
+              make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(&bar.q_full[half]);
+      const int lim_all = row_limit(p, it.q, it.row_lo + it.rows - 1);
+      const int lim = live ? row_limit(p, it.q, row) : lim_all;
+      const int lim_warp = row_limit(p, it.q, it.row_lo + min(it.rows - 1, half * 128 + quarter * 32));
+      float m = -INFINITY, l = 0.f;  // reference of the weights, sum
+      // scale exponents of a tile's four 32-position blocks: lanes 0-3
+      int sc = 0, sc_next = 0;
+      auto get_scales = [&](int64_t tile) {
+        int e = 127 | 127 << 8;
+        const int64_t pos = tile * TILE + 32 * (lane & 3);
+        if (KV == KV_E4M3 && pos < lim_all) {
+          int64_t page = p.b.table[it.seq * p.b.max_pages + pos / p.pg.page_size];
+          if (page < 0 || page >= p.pg.n_pages) page = 0;
+          const int64_t at = kv_row(p.pg, page, w.head, (int)(pos % p.pg.page_size)) / kScaleBlock;
+          e = p.pg.k_scale[at] | p.pg.v_scale[at] << 8;
+        }
+        return e;
+      };
+      sc_next = get_scales(w.tile0);
+      for (int64_t t = w.tile0; t < w.tile1; ++t) {
+        sc = sc_next;
+        if (t + 1 < w.tile1) sc_next = get_scales(t + 1);
+        float c[4], ev[4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          const int e = __shfl_sync(0xffffffffu, sc, b);
+          c[b] = KV == KV_E4M3 ? factor * pow2i((e & 255) - 127) : factor;
+          ev[b] = KV == KV_E4M3 ? (float)((e >> 8) - 127) : 0.f;
+        }
+        ok = warp_wait(&bar.s_full[half], ph_s, err, kTimeout);
+        if (!ok) break;
+        ph_s ^= 1;
+        tc_fence_after();
+        const int valid = (int)min((int64_t)TILE, max((int64_t)0, lim - t * TILE));  // columns this row sees
+        const bool edge = (t + 1) * TILE > lim_warp;
+        float mx = -INFINITY;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          uint32_t x[32];
+          tmem_ld32(s_addr + 32 * b, x);
+          tmem_wait_ld();
+          float top = -INFINITY;
+          if (edge) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) top = fmaxf(top, 32 * b + i < valid ? __uint_as_float(x[i]) : -INFINITY);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) top = fmaxf(top, __uint_as_float(x[i]));
+          }
+          mx = fmaxf(mx, fmaf(top, c[b], ev[b]));
+        }
+        float shrink = 1.f;
+        if (mx > m + 8.f || m == -INFINITY) {
+          const float to = fmaxf(m, mx);
+          shrink = to == -INFINITY ? 1.f : ex2(m - to);
+          m = to;
+          l *= shrink;
+        }
+        if (t > w.tile0 && __any_sync(0xffffffffu, shrink != 1.f)) {
+          // the products of the tile before have ended: the scores' arrival counts them
+#pragma unroll 1
+          for (int d = 0; d < HD; d += 16) {
+            uint32_t x[16];
+            tmem_ld16(o_addr + d, x);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * shrink);
+            tmem_st16(o_addr + d, x);
+          }
+        }
+        const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          uint32_t x[32];
+          tmem_ld32(s_addr + 32 * b, x);
+          tmem_wait_ld();
+          const float off = ev[b] - base;
+          float sum = 0.f;
+          uint32_t pk[16];
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            float a = fmaf(__uint_as_float(x[i]), c[b], off), d = fmaf(__uint_as_float(x[i + 1]), c[b], off);
+            if (edge) {
+              a = 32 * b + i < valid ? a : -INFINITY;
+              d = 32 * b + i + 1 < valid ? d : -INFINITY;
+            }
+            a = ex2(a), d = ex2(d);
+            sum += a + d;
+            pk[i / 2] = pack2<kBf>(a, d);
+          }
+          l = fmaf(sum, KV == KV_E4M3 ? pow2i(-(int)ev[b]) : 1.f, l);
+          tmem_st16(s_addr + 16 * b, pk);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&bar.p_full[half]);
+      }
+      if (!ok) break;
+      ok = warp_wait(&bar.o_full[half], ph_o, err, kTimeout);
+      if (!ok) break;
+      ph_o ^= 1;
+      tc_fence_after();
+      const bool marked = *const_cast<volatile int*>(&any_not_finite[w.seg & 3]) != 0;
+      float* part = p.part + (int64_t)(2 * blockIdx.x + (w.tile0 == 0 ? 1 : 0)) * C::kPart;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const int64_t at = (int64_t)(it.q.row0 + row / p.group) * p.out_stride + (int64_t)(w.head * p.group + row % p.group) * HD;
+#pragma unroll 1
+      for (int d = 0; d < HD; d += 16) {
+        uint32_t x[16];
+        tmem_ld16(o_addr + d, x);
+        tmem_wait_ld();
+        if (marked) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (*const_cast<volatile int*>(&not_finite_from[w.seg & 3][d + i]) < lim) x[i] = 0x7fc00000u;
+        }
+        if (!live) continue;
+        if (whole) {
+          uint32_t h[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float a = l == 0.f ? 0.f : __uint_as_float(x[2 * i]) * inv, b = l == 0.f ? 0.f : __uint_as_float(x[2 * i + 1]) * inv;
+            h[i] = p.is_bf16 ? pack2<true>(a, b) : pack2<false>(a, b);
+          }
+          if (p.vec_out16) {
+            reinterpret_cast<uint4*>(p.out + at + d)[0] = make_uint4(h[0], h[1], h[2], h[3]);
+            reinterpret_cast<uint4*>(p.out + at + d)[1] = make_uint4(h[4], h[5], h[6], h[7]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) p.out[at + d + i] = (uint16_t)(h[i / 2] >> (16 * (i & 1)));
+          }
+        } else {
+          float4* to = reinterpret_cast<float4*>(part + my * HD + d);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            to[i] = make_float4(__uint_as_float(x[4 * i]), __uint_as_float(x[4 * i + 1]), __uint_as_float(x[4 * i + 2]),
+                                __uint_as_float(x[4 * i + 3]));
+        }
+      }
+      if (live) {
+        if (whole)
+          store_lse(p, it.q, row, w.head, m, l);
+        else
+          part[R * HD + 2 * my] = m, part[R * HD + 2 * my + 1] = l;
+      }
+      tc_fence_before();
+      mbar_arrive(&bar.read[w.seg & 3]);
+    }
+    if (tid == 0) p.desc[blockIdx.x] = begun;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 12) tmem_dealloc(tmem, 512);
+  pdl_trigger();
+}
+
 // Adds the partial triples of the item that CTA blockIdx.x of the first kernel began: those of
-// slots 2c + 1, 2(c + 1), .. 2 last, in that order. One CTA a row: 8 groups of HD / 4 threads.. take every
-// eighth triple, then their sums are added in order.
-template <int HD, int R, int TILE>
+// slots 2c + 1, 2(c + 1), .. 2 last. HD / 4 threads a row; GROUPS of them share the triples of one row and
+// add their sums in order (few rows: many triples each), or take a row each (GROUPS = 1).
+template <int HD, int R, int TILE, int GROUPS>
 __global__ void __launch_bounds__(8 * HD / 4) kv_combine_kernel(const __grid_constant__ AttnParams p) {
-  constexpr int kLanes = HD / 4;
+  constexpr int kLanes = HD / 4, kRows = 8 / GROUPS;
   __shared__ float4 acc_s[8][kLanes];
   __shared__ float l_s[8];
   pdl_wait();
-  const int c = blockIdx.x, r = blockIdx.y;
+  const int c = blockIdx.x;
   const int4 begun = p.desc[c];
   if (begun.w == 0) return;
   const Item it = item_of<R, TILE>(p, begun.x);
-  if (r >= it.rows) return;
-  const int n = begun.z - c + 1;
-  const int sub = threadIdx.x % kLanes, grp = threadIdx.x / kLanes;
+  const int sub = threadIdx.x % kLanes, team = threadIdx.x / kLanes, grp = team % GROUPS;
+  const int r = blockIdx.y * kRows + team / GROUPS;
+  if (blockIdx.y * kRows >= it.rows) return;
+  const bool live = r < it.rows;
+  const int n = live ? begun.z - c + 1 : 0;
   auto slot = [&](int k) { return p.part + (int64_t)(2 * (c + k) + (k == 0 ? 1 : 0)) * (R * (HD + 2)); };
   float m = -INFINITY;
   for (int k = 0; k < n; ++k) m = fmaxf(m, slot(k)[R * HD + 2 * r]);
   const float base = m == -INFINITY ? 0.f : m;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   float l = 0.f;
-  for (int k = grp; k < n; k += 8) {
+  for (int k = grp; k < n; k += GROUPS) {
     const float* s = slot(k);
     const float f = ex2(s[R * HD + 2 * r] - base);
     const float4 v = reinterpret_cast<const float4*>(s + r * HD)[sub];
     acc.x = fmaf(v.x, f, acc.x), acc.y = fmaf(v.y, f, acc.y), acc.z = fmaf(v.z, f, acc.z), acc.w = fmaf(v.w, f, acc.w);
     l = fmaf(s[R * HD + 2 * r + 1], f, l);
   }
-  acc_s[grp][sub] = acc;
-  if (sub == 0) l_s[grp] = l;
-  __syncthreads();
-  if (grp != 0) return;
-  for (int k = 1; k < 8; ++k) {
-    const float4 v = acc_s[k][sub];
-    acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
-    l += l_s[k];
+  if (GROUPS > 1) {
+    acc_s[team][sub] = acc;
+    if (sub == 0) l_s[team] = l;
+    __syncthreads();
+    if (grp != 0) return;
+    for (int k = 1; k < GROUPS; ++k) {
+      const float4 v = acc_s[team + k][sub];
+      acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+      l += l_s[team + k];
+    }
   }
+  if (!live) return;
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const float x[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
 #pragma unroll
@@ -640,7 +1262,9 @@ __global__ void __launch_bounds__(8 * HD / 4) kv_combine_kernel(const __grid_con
 // host
 // ---------------------------------------------------------------------------------------------
 constexpr int kRowsGrid = 148;
+constexpr int kTileGrid = 148;
 constexpr int kMaxGrid = 148;
+constexpr int kRowsMax = 16;  // rows of a sequence and key/value head that the few-rows kernel takes
 
 template <int HD, int KV, int NT>
 cudaError_t launch_rows(AttnParams p, int max_rows, cudaStream_t st) {
@@ -653,17 +1277,43 @@ cudaError_t launch_rows(AttnParams p, int max_rows, cudaStream_t st) {
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   set_pdl_for_call(true);
-  e = launch_pdl(kv_combine_kernel<HD, C::R, C::TILE>, dim3(kRowsGrid, C::R), dim3(8 * HD / 4), 0, st, p);
+  e = launch_pdl(kv_combine_kernel<HD, C::R, C::TILE, 8>, dim3(kRowsGrid, C::R), dim3(8 * HD / 4), 0, st, p);
+  set_pdl_for_call(false);
+  return e;
+}
+
+template <int HD, int KV>
+cudaError_t launch_tiles(AttnParams p, int max_rows, cudaStream_t st) {
+  using C = TileCfg<HD, KV>;
+  p.n_qt = (max_rows + C::R - 1) / C::R;
+  static_assert(C::kSmem <= 220 * 1024, "shared memory");
+  cudaError_t e = cudaFuncSetAttribute(kv_tile_kernel<HD, KV>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmem);
+  if (e != cudaSuccess) return e;
+  kv_tile_kernel<HD, KV><<<kTileGrid, C::kThreads, C::kSmem, st>>>(p);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  set_pdl_for_call(true);
+  e = launch_pdl(kv_combine_kernel<HD, C::R, C::TILE, 1>, dim3(kTileGrid, C::R / 8), dim3(8 * HD / 4), 0, st, p);
   set_pdl_for_call(false);
   return e;
 }
 
 template <int HD, int KV>
 cudaError_t launch_kv(const AttnParams& p, int max_rows, cudaStream_t st) {
-  return max_rows <= 8 ? launch_rows<HD, KV, 1>(p, max_rows, st) : launch_rows<HD, KV, 2>(p, max_rows, st);
+  return max_rows <= 8          ? launch_rows<HD, KV, 1>(p, max_rows, st)
+         : max_rows <= kRowsMax ? launch_rows<HD, KV, 2>(p, max_rows, st)
+                                : launch_tiles<HD, KV>(p, max_rows, st);
 }
 
-size_t workspace_bytes_of(int hd) { return (size_t)kMaxGrid * (2 * 16 * (hd + 2) * 4 + sizeof(int4)); }
+// desc, the waits' error word, partial triples (two a CTA) of the larger row tile that max_rows can need
+constexpr size_t kWsHead = kMaxGrid * sizeof(int4) + 16;
+size_t workspace_bytes_of(int hd, int64_t max_rows) {
+  const int64_t rows = max_rows <= kRowsMax ? kRowsMax : 256;
+  return kWsHead + (size_t)kMaxGrid * 2 * rows * (hd + 2) * 4;
+}
+int64_t max_rows_of(const dmoe_kv_cache* c, const dmoe_kv_batch* b, const dmoe_kv_attention_args* a) {
+  return std::min<int64_t>(b->max_q_len, a->n_tokens) * (a->n_head / std::max(1, c->n_head_kv));
+}
 
 }  // namespace
 
@@ -674,7 +1324,7 @@ using namespace dmoe;
 extern "C" size_t dmoe_kv_attention_workspace(const dmoe_kv_cache* cache, const dmoe_kv_batch* batch,
                                               const dmoe_kv_attention_args* a) {
   if (!cache || !batch || !a || (cache->head_dim != 64 && cache->head_dim != 128)) return 0;
-  return workspace_bytes_of(cache->head_dim);
+  return workspace_bytes_of(cache->head_dim, max_rows_of(cache, batch, a));
 }
 
 extern "C" dmoe_status dmoe_kv_attention(const dmoe_kv_cache* cache, const dmoe_kv_batch* batch,
@@ -720,10 +1370,13 @@ extern "C" dmoe_status dmoe_kv_attention(const dmoe_kv_cache* cache, const dmoe_
   p.group = group;
   p.block_length = a->block_length;
   p.vec_q = ((reinterpret_cast<uintptr_t>(a->q) | (uintptr_t)(2 * a->q_stride)) & 7u) == 0;
+  p.vec_q16 = ((reinterpret_cast<uintptr_t>(a->q) | (uintptr_t)(2 * a->q_stride)) & 15u) == 0;
+  p.vec_out16 = ((reinterpret_cast<uintptr_t>(a->out) | (uintptr_t)(2 * a->out_stride)) & 15u) == 0;
   p.scale_log2 = a->scale * kLog2e;
   p.desc = static_cast<int4*>(workspace);
-  p.part = reinterpret_cast<float*>(p.desc + kMaxGrid);
-  const int max_rows = (int)std::min<int64_t>(batch->max_q_len, a->n_tokens) * group;
+  p.wait_err = cache->err ? cache->err : reinterpret_cast<uint32_t*>(p.desc + kMaxGrid);
+  p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kWsHead);
+  const int max_rows = (int)max_rows_of(cache, batch, a);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const KvType kv = kv_type_of(cache->type);
   cudaError_t e;

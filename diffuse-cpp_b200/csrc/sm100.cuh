@@ -204,6 +204,18 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
       : "memory");
 }
 
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+
 // ---------------------------------------------------------------------------------------------
 // tcgen05: MMA (kind::f16, fp16 x fp16 -> fp32 accumulators in TMEM)
 // ---------------------------------------------------------------------------------------------
@@ -213,6 +225,12 @@ __host__ __device__ constexpr uint32_t idesc_f16_f32(uint32_t M, uint32_t N) {
          | (0u << 7) | (0u << 10)  // A, B = f16
          | (0u << 15) | (0u << 16) // K-major A and B
          | ((N >> 3) << 17) | ((M >> 4) << 24);
+}
+
+// The same for operands of either 16-bit type (A and B alike), with B K-major or MN-major.
+__host__ __device__ constexpr uint32_t idesc_16b_f32(uint32_t M, uint32_t N, bool bf16, bool b_mn_major) {
+  return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((b_mn_major ? 1u : 0u) << 16) |
+         ((N >> 3) << 17) | ((M >> 4) << 24);
 }
 
 // Shared-memory matrix descriptor, K-major, 128-byte swizzle: 8-row x 128-byte atoms stacked
@@ -225,6 +243,18 @@ __device__ __forceinline__ uint64_t sdesc_sw128(uint32_t saddr, uint32_t sbo_byt
   d |= (uint64_t)((sbo_bytes >> 4) & 0x3FFFu) << 32;    // SBO
   d |= (uint64_t)1u << 46;                              // descriptor version (sm100)
   d |= (uint64_t)2u << 61;                              // SWIZZLE_128B
+  return d;
+}
+
+// MN-major, 128-byte swizzle: rows of K, 64 elements of M/N in each 128-byte row, 8-row atoms every
+// 1024 bytes along K; the next 64 elements of M/N `lbo_bytes` on. 16 K are 2048 bytes.
+__device__ __forceinline__ uint64_t sdesc_sw128_mn(uint32_t saddr, uint32_t lbo_bytes) {
+  uint64_t d = 0;
+  d |= (uint64_t)((saddr >> 4) & 0x3FFFu);
+  d |= (uint64_t)((lbo_bytes >> 4) & 0x3FFFu) << 16;
+  d |= (uint64_t)((1024u >> 4) & 0x3FFFu) << 32;
+  d |= (uint64_t)1u << 46;
+  d |= (uint64_t)2u << 61;
   return d;
 }
 
