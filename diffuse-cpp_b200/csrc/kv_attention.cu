@@ -344,12 +344,13 @@ __global__ void __launch_bounds__(256, 1) kv_rows_kernel(const __grid_constant__
     int ek = 0, ev = 0;
     // page of a step's positions (a step lies in one scale block, so in one page), scales and keys
     auto load_keys = [&](int at_pos) {
-      int64_t page = table[at_pos / p.pg.page_size];
+      const uint32_t blk = (uint32_t)at_pos / kScaleBlock, slot = kv_slot(p.pg, blk);
+      int64_t page = table[slot];
       if (page < 0 || page >= p.pg.n_pages) {
         kv_report(p.pg.err, DMOE_KV_ERR_PAGE);
         page = 0;
       }
-      row = kv_row(p.pg, page, head, at_pos % p.pg.page_size);
+      row = kv_row(p.pg, page, head, (int)(blk - slot * p.pg.page_blocks) * kScaleBlock + at_pos % kScaleBlock);
       if (KV == KV_E4M3) {
         ek = (int)p.pg.k_scale[row / kScaleBlock] - 127;
         ev = (int)p.pg.v_scale[row / kScaleBlock] - 127;
@@ -782,25 +783,34 @@ __global__ void __launch_bounds__(416, 1) kv_tile_kernel(const __grid_constant__
     const int c = lt % LPR, r0 = lt / LPR;
     uint32_t kv_n = 0;
     bool ok = true;
-    int pages[4];  // of the tile's 32-position groups
-    auto get_pages = [&](const Item& it, int64_t tile, int lim) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int64_t pos = tile * TILE + 32 * i;
-        pages[i] = 0;
-        if (pos < lim) {
-          pages[i] = p.b.table[it.seq * p.b.max_pages + pos / p.pg.page_size];
-          if (pages[i] < 0 || pages[i] >= p.pg.n_pages) {
+    // first row of each of the tile's 32-position blocks in the pages. The page numbers of eight tiles
+    // are read at once, one a lane
+    int64_t first_row[4];
+    int held = 0, held_from = 0, held_to = 0;  // blocks [held_from, held_to) of the item
+    auto get_pages = [&](const Item& it, int head, int tile, int lim, bool new_item) {
+      const int b0 = tile * (TILE / 32);
+      if (new_item || b0 >= held_to) {
+        held_from = b0, held_to = b0 + 32;
+        held = 0;
+        if ((b0 + lane) * 32 < lim) {
+          held = p.b.table[it.seq * p.b.max_pages + kv_slot(p.pg, b0 + lane)];
+          if (held < 0 || held >= p.pg.n_pages) {
             kv_report(p.pg.err, DMOE_KV_ERR_PAGE);
-            pages[i] = 0;
+            held = 0;
           }
         }
       }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int page = __shfl_sync(0xffffffffu, held, b0 + i - held_from);
+        const uint32_t b = b0 + i;
+        first_row[i] = kv_row(p.pg, page, head, (int)(b - kv_slot(p.pg, b) * p.pg.page_blocks) * kScaleBlock);
+      }
     };
-    // byte offset of row r of the tile, at this thread's piece
-    auto source = [&](int head, int64_t tile, int r) {
-      const int off = (int)((tile * TILE + (r & ~31)) % p.pg.page_size) + (r & 31);
-      return kv_row(p.pg, pages[r >> 5], head, off) * (HD * ES) + 16 * c;
+    // byte offset of this thread's i-th piece of the tile; its row is r0 + i * RPI
+    auto source = [&](int i) {
+      const int r = r0 + i * RPI;
+      return (first_row[i * RPI / 32] + (r & 31)) * (HD * ES) + 16 * c;
     };
     // positions that only some rows see, and values that are not finite there: their products with a zero
     // weight would reach the others. They are set to zero, and their element marked for the rows that see them
@@ -818,12 +828,12 @@ __global__ void __launch_bounds__(416, 1) kv_tile_kernel(const __grid_constant__
     };
     if constexpr (KV == KV_E4M3) {
       uint4 kr[N], vr[N];
-      auto fetch = [&](uint4 (&x)[N], const void* base, int head, int64_t tile, int lim) {
+      auto fetch = [&](uint4 (&x)[N], const void* base, int tile, int lim) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
           const int r = r0 + i * RPI;
           x[i] = make_uint4(0, 0, 0, 0);
-          if (tile * TILE + r < lim) x[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(base) + source(head, tile, r)));
+          if (tile * TILE + r < lim) x[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(base) + source(i)));
         }
       };
       auto put = [&](const uint4 (&x)[N], uint8_t* dst) {
@@ -844,18 +854,18 @@ __global__ void __launch_bounds__(416, 1) kv_tile_kernel(const __grid_constant__
       };
       if (w.more()) {
         const int lim = row_limit(p, w.it.q, w.it.row_lo + w.it.rows - 1);
-        get_pages(w.it, w.tile0, lim);
-        fetch(kr, p.pg.k, w.head, w.tile0, lim);
-        fetch(vr, p.pg.v, w.head, w.tile0, lim);
+        get_pages(w.it, w.head, (int)w.tile0, lim, true);
+        fetch(kr, p.pg.k, (int)w.tile0, lim);
+        fetch(vr, p.pg.v, (int)w.tile0, lim);
       }
       while (ok && w.more()) {
         const int lim_min = row_limit(p, w.it.q, w.it.row_lo);
         const int lim_max = row_limit(p, w.it.q, w.it.row_lo + w.it.rows - 1);
         const int seg = w.seg, head = w.head;
         const Item it = w.it;
-        const int64_t t0 = w.tile0, t1 = w.tile1;
+        const int t0 = (int)w.tile0, t1 = (int)w.tile1;
         w.next();
-        for (int64_t t = t0; t < t1; ++t, ++kv_n) {
+        for (int t = t0; t < t1; ++t, ++kv_n) {
           const int stage = kv_n & 1;
           const uint32_t ph = ((kv_n >> 1) & 1) ^ 1;
           ok = warp_wait(&bar.k_empty[stage], ph, err, kTimeout);
@@ -867,11 +877,11 @@ __global__ void __launch_bounds__(416, 1) kv_tile_kernel(const __grid_constant__
           const bool same = t + 1 < t1, more = same || w.more();
           const Item& ni = same ? it : w.it;
           const int nh = same ? head : w.head;
-          const int64_t nt = same ? t + 1 : w.tile0;
+          const int nt = same ? t + 1 : (int)w.tile0;
           const int nl = same ? lim_max : more ? row_limit(p, w.it.q, w.it.row_lo + w.it.rows - 1) : 0;
           if (more) {
-            get_pages(ni, nt, nl);
-            fetch(kr, p.pg.k, nh, nt, nl);
+            get_pages(ni, nh, nt, nl, !same);
+            fetch(kr, p.pg.k, nt, nl);
           }
           ok = warp_wait(&bar.v_empty[stage], ph, err, kTimeout);
           if (!ok) break;
@@ -882,7 +892,7 @@ __global__ void __launch_bounds__(416, 1) kv_tile_kernel(const __grid_constant__
           if (lim_min < lim_max && (t + 1) * TILE > lim_min) {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-              const int pos = (int)(t * TILE) + r0 + i * RPI;
+              const int pos = t * TILE + r0 + i * RPI;
               uint32_t v[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
@@ -899,17 +909,17 @@ __global__ void __launch_bounds__(416, 1) kv_tile_kernel(const __grid_constant__
           put(vr, v_s + stage * C::kOperand);
           fence_proxy_async_smem();
           mbar_arrive(&bar.v_full[stage]);
-          if (more) fetch(vr, p.pg.v, nh, nt, nl);
+          if (more) fetch(vr, p.pg.v, nt, nl);
         }
       }
     } else {
       // 16-bit pages need no conversion: asynchronous copies, the next tile's keys ahead of this one's arrival
-      auto issue = [&](const void* base, uint8_t* dst, int head, int64_t tile, int lim) {
+      auto issue = [&](const void* base, uint8_t* dst, int tile, int lim) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
           const int r = r0 + i * RPI;
           const bool in = tile * TILE + r < lim;
-          const uint8_t* src = static_cast<const uint8_t*>(base) + (in ? source(head, tile, r) : 0);
+          const uint8_t* src = static_cast<const uint8_t*>(base) + (in ? source(i) : 0);
           const uint32_t to = smem_u32(dst) + (c / 8) * C::kPlane + r * 128 + 16 * ((c % 8) ^ (r & 7));
           asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(src), "r"(in ? 16 : 0) : "memory");
         }
@@ -917,30 +927,30 @@ __global__ void __launch_bounds__(416, 1) kv_tile_kernel(const __grid_constant__
       };
       if (w.more()) {
         const int lim = row_limit(p, w.it.q, w.it.row_lo + w.it.rows - 1);
-        get_pages(w.it, w.tile0, lim);
-        issue(p.pg.k, k_s, w.head, w.tile0, lim);  // the ring is empty
-        issue(p.pg.v, v_s, w.head, w.tile0, lim);
+        get_pages(w.it, w.head, (int)w.tile0, lim, true);
+        issue(p.pg.k, k_s, (int)w.tile0, lim);  // the ring is empty
+        issue(p.pg.v, v_s, (int)w.tile0, lim);
       }
       while (ok && w.more()) {
         const int lim_min = row_limit(p, w.it.q, w.it.row_lo);
         const int lim_max = row_limit(p, w.it.q, w.it.row_lo + w.it.rows - 1);
         const int seg = w.seg, head = w.head;
         const Item it = w.it;
-        const int64_t t0 = w.tile0, t1 = w.tile1;
+        const int t0 = (int)w.tile0, t1 = (int)w.tile1;
         w.next();
-        for (int64_t t = t0; t < t1; ++t, ++kv_n) {
+        for (int t = t0; t < t1; ++t, ++kv_n) {
           const int stage = kv_n & 1, next = (kv_n + 1) & 1;
           const uint32_t ph = (((kv_n + 1) >> 1) & 1) ^ 1;
           const bool same = t + 1 < t1, more = same || w.more();
           const Item& ni = same ? it : w.it;
           const int nh = same ? head : w.head;
-          const int64_t nt = same ? t + 1 : w.tile0;
+          const int nt = same ? t + 1 : (int)w.tile0;
           const int nl = same ? lim_max : more ? row_limit(p, w.it.q, w.it.row_lo + w.it.rows - 1) : 0;
           if (more) {
-            get_pages(ni, nt, nl);
+            get_pages(ni, nh, nt, nl, !same);
             ok = warp_wait(&bar.k_empty[next], ph, err, kTimeout);
             if (!ok) break;
-            issue(p.pg.k, k_s + next * C::kOperand, nh, nt, nl);
+            issue(p.pg.k, k_s + next * C::kOperand, nt, nl);
             asm volatile("cp.async.wait_group 1;" ::: "memory");
           } else {
             asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -952,7 +962,7 @@ __global__ void __launch_bounds__(416, 1) kv_tile_kernel(const __grid_constant__
           if (lim_min < lim_max && (t + 1) * TILE > lim_min) {
 #pragma unroll 1
             for (int i = 0; i < N; ++i) {
-              const int r = r0 + i * RPI, pos = (int)(t * TILE) + r;
+              const int r = r0 + i * RPI, pos = t * TILE + r;
               uint4* at = reinterpret_cast<uint4*>(v_s + stage * C::kOperand + (c / 8) * C::kPlane + r * 128 + 16 * ((c % 8) ^ (r & 7)));
               const uint4 x = *at;  // this thread's own copy
               uint32_t v[4] = {x.x, x.y, x.z, x.w};
@@ -977,7 +987,7 @@ __global__ void __launch_bounds__(416, 1) kv_tile_kernel(const __grid_constant__
           if (more) {
             ok = warp_wait(&bar.v_empty[next], ph, err, kTimeout);
             if (!ok) break;
-            issue(p.pg.v, v_s + next * C::kOperand, nh, nt, nl);
+            issue(p.pg.v, v_s + next * C::kOperand, nt, nl);
           }
         }
       }
@@ -1058,21 +1068,23 @@ __global__ void __launch_bounds__(416, 1) kv_tile_kernel(const __grid_constant__
       float m = -INFINITY, l = 0.f;  // reference of the weights, sum
       // scale exponents of a tile's four 32-position blocks: lanes 0-3
       int sc = 0, sc_next = 0;
-      auto get_scales = [&](int64_t tile) {
+      auto get_scales = [&](int tile) {
         int e = 127 | 127 << 8;
-        const int64_t pos = tile * TILE + 32 * (lane & 3);
-        if (KV == KV_E4M3 && pos < lim_all) {
-          int64_t page = p.b.table[it.seq * p.b.max_pages + pos / p.pg.page_size];
+        const uint32_t b = tile * (TILE / 32) + (lane & 3);
+        if (KV == KV_E4M3 && (int)b * 32 < lim_all) {
+          const uint32_t slot = kv_slot(p.pg, b);
+          int64_t page = p.b.table[it.seq * p.b.max_pages + slot];
           if (page < 0 || page >= p.pg.n_pages) page = 0;
-          const int64_t at = kv_row(p.pg, page, w.head, (int)(pos % p.pg.page_size)) / kScaleBlock;
+          const int64_t at = (page * p.pg.n_head_kv + w.head) * p.pg.page_blocks + (b - slot * p.pg.page_blocks);
           e = p.pg.k_scale[at] | p.pg.v_scale[at] << 8;
         }
         return e;
       };
-      sc_next = get_scales(w.tile0);
-      for (int64_t t = w.tile0; t < w.tile1; ++t) {
+      const int t0 = (int)w.tile0, t1 = (int)w.tile1;
+      sc_next = get_scales(t0);
+      for (int t = t0; t < t1; ++t) {
         sc = sc_next;
-        if (t + 1 < w.tile1) sc_next = get_scales(t + 1);
+        if (t + 1 < t1) sc_next = get_scales(t + 1);
         float c[4], ev[4];
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
@@ -1084,7 +1096,7 @@ __global__ void __launch_bounds__(416, 1) kv_tile_kernel(const __grid_constant__
         if (!ok) break;
         ph_s ^= 1;
         tc_fence_after();
-        const int valid = (int)min((int64_t)TILE, max((int64_t)0, lim - t * TILE));  // columns this row sees
+        const int valid = min(TILE, max(0, lim - t * TILE));  // columns this row sees
         const bool edge = (t + 1) * TILE > lim_warp;
         float mx = -INFINITY;
 #pragma unroll
@@ -1109,7 +1121,7 @@ __global__ void __launch_bounds__(416, 1) kv_tile_kernel(const __grid_constant__
           m = to;
           l *= shrink;
         }
-        if (t > w.tile0 && __any_sync(0xffffffffu, shrink != 1.f)) {
+        if (t > t0 && __any_sync(0xffffffffu, shrink != 1.f)) {
           // the products of the tile before have ended: the scores' arrival counts them
 #pragma unroll 1
           for (int d = 0; d < HD; d += 16) {

@@ -24,7 +24,15 @@ struct KvPages {
   uint32_t* err;
   int64_t n_pages;
   int n_head_kv, page_size;
+  int page_blocks;       // page_size / 32
+  uint64_t page_magic;   // ceil(2^36 / page_blocks)
 };
+
+// Page slot of 32-position block b, b < 2^25 (positions are below 2^30): b / page_blocks, exactly, since
+// page_blocks <= 2^11 and b * (page_magic * page_blocks - 2^36) < 2^36.
+__device__ __forceinline__ uint32_t kv_slot(const KvPages& pg, uint32_t b) {
+  return (uint32_t)((b * pg.page_magic) >> 36);
+}
 
 struct KvBatch {
   const int32_t* table;
@@ -68,7 +76,9 @@ inline KvType kv_type_of(int type) {
   return type == DMOE_TYPE_BF16 ? KV_BF16 : type == DMOE_TYPE_F16 ? KV_F16 : KV_E4M3;
 }
 inline KvPages kv_pages(const dmoe_kv_cache* c) {
-  return {c->k, c->v, c->k_scale, c->v_scale, c->err, c->n_pages, c->n_head_kv, c->page_size};
+  const uint64_t blocks = (uint64_t)c->page_size / kScaleBlock;
+  return {c->k, c->v, c->k_scale, c->v_scale, c->err, c->n_pages, c->n_head_kv, c->page_size, (int)blocks,
+          ((uint64_t{1} << 36) + blocks - 1) / blocks};
 }
 inline KvBatch kv_batch(const dmoe_kv_batch* b, int64_t n_tokens) {
   return {b->page_table, b->q_start, b->kv_len, b->max_pages, n_tokens, b->n_seq, b->max_q_len};
