@@ -86,23 +86,28 @@ __device__ __forceinline__ Item item_of(const AttnParams& p, int u) {
   return it;
 }
 
-struct Run {       // a CTA's run of tiles
+// Beginning and ending an item costs about as much as OV tiles. An item of t tiles is OV + t units long, and
+// the units of all items are numbered through; its tiles are the last t.
+struct Run {       // a CTA's run of units
   int u, head;     // first item
-  int64_t tile;    // first tile within it
-  int64_t left;    // tiles of the run
-  int64_t chunk;   // tiles of every run but the last
-  int64_t first;   // number of the first tile
+  int unit;        // first unit within it
+  int left;        // units of the run (2^31 tiles would take an hour: no workload has them)
+  int chunk;       // units of every run but the last
+  int64_t first;   // number of the first unit
 };
 
 // The whole CTA: finds its run. smem: scratch of THREADS / 32 + 1 words and one Run.
-template <int R, int TILE, int THREADS>
+template <int R, int TILE, int OV, int THREADS>
 __device__ __forceinline__ Run find_run(const AttnParams& p, int64_t* sums, Run* found) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t n_u = (int64_t)p.b.n_seq * p.n_qt;
   const int64_t per = (n_u + THREADS - 1) / THREADS;
   const int64_t u0 = min(n_u, per * tid), u1 = min(n_u, u0 + per);
   int64_t mine = 0;
-  for (int64_t u = u0; u < u1; ++u) mine += item_of<R, TILE>(p, (int)u).tiles;
+  for (int64_t u = u0; u < u1; ++u) {
+    const int t = item_of<R, TILE>(p, (int)u).tiles;
+    if (t) mine += t + OV;
+  }
   int64_t incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -119,17 +124,18 @@ __device__ __forceinline__ Run find_run(const AttnParams& p, int64_t* sums, Run*
   }
   const int heads = p.pg.n_head_kv;
   total *= heads;
-  const int64_t chunk = (total + gridDim.x - 1) / gridDim.x;
+  const int64_t chunk = min((total + gridDim.x - 1) / gridDim.x, (int64_t)INT32_MAX);
   const int64_t first = chunk * blockIdx.x;
   before *= heads;
   if (first < total && first >= before && first < before + mine * heads) {
     for (int64_t u = u0; u < u1; ++u) {
-      const int64_t w = item_of<R, TILE>(p, (int)u).tiles;
+      const int t = item_of<R, TILE>(p, (int)u).tiles;
+      const int64_t w = t ? t + OV : 0;
       if (first < before + w * heads) {
         found->u = (int)u;
         found->head = (int)((first - before) / w);
-        found->tile = (first - before) % w;
-        found->left = min(chunk, total - first);
+        found->unit = (int)((first - before) % w);
+        found->left = (int)min(chunk, total - first);
         break;
       }
       before += w * heads;
@@ -137,10 +143,58 @@ __device__ __forceinline__ Run find_run(const AttnParams& p, int64_t* sums, Run*
   }
   __syncthreads();
   Run r = *found;
-  r.chunk = chunk;
+  r.chunk = (int)chunk;
   r.first = first;
   return r;
 }
+
+// Walks a CTA's run, item by item: every warp role does it on its own. The segment at hand is the tiles
+// [t0, t1) of `it`; an item of which the run only holds units before its tiles is left to the next CTA.
+template <int R, int TILE, int OV>
+struct Walk {
+  const AttnParams& p;
+  Item it{};
+  int u, head, seg = -1, t0 = 0, t1 = 0;
+  int unit, left, chunk;
+  int64_t at;
+  __device__ __forceinline__ Walk(const AttnParams& p_, const Run& r)
+      : p(p_), u(r.u), head(r.head), unit(r.unit), left(r.left), chunk(r.chunk), at(r.first) {
+    if (left > 0) it = item_of<R, TILE>(p, u);
+    settle();
+  }
+  __device__ __forceinline__ bool more() const { return left > 0; }
+  __device__ __forceinline__ bool whole() const { return t0 == 0 && t1 == it.tiles; }
+  // {item, head, last CTA that has a part of it, 1}: for an item that this CTA begins and does not end
+  __device__ __forceinline__ int4 begun() const {
+    return make_int4(u, head, (int)((at - unit + OV + it.tiles - 1) / chunk), 1);
+  }
+  __device__ __forceinline__ void next() {
+    advance();
+    settle();
+  }
+
+ private:
+  __device__ __forceinline__ void advance() {
+    const int n = min(left, OV + it.tiles - unit);
+    left -= n;
+    at += n;
+    unit = 0;
+    if (left > 0 && ++head == p.pg.n_head_kv) {
+      head = 0;
+      do it = item_of<R, TILE>(p, ++u);
+      while (it.tiles == 0);
+    }
+  }
+  __device__ __forceinline__ void settle() {
+    while (left > 0) {
+      t0 = max(0, unit - OV);
+      t1 = (int)min((int64_t)it.tiles, (int64_t)unit + left - OV);
+      if (t1 > t0) break;
+      advance();
+    }
+    ++seg;
+  }
+};
 
 // ---------------------------------------------------------------------------------------------
 // 16-bit warp products
@@ -255,6 +309,7 @@ struct RowsCfg {
   static constexpr int MT = KV == KV_E4M3 ? 2 : 1;  // 16-position product tiles a step
   static constexpr int STEP = 16 * MT;
   static constexpr int TILE = kWarps * STEP;
+  static constexpr int OV = 1;
   static constexpr int ES = KV == KV_E4M3 ? 1 : 2;
   static constexpr size_t kSmem = (size_t)kWarps * R * (HD + 2) * 4;
   static constexpr int kPart = R * (HD + 2);  // floats of a partial triple
@@ -274,15 +329,11 @@ __global__ void __launch_bounds__(256, 1) kv_rows_kernel(const __grid_constant__
   __shared__ Run found;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
 
-  Run run = find_run<R, TILE, 256>(p, sums, &found);
+  pdl_wait();
   int4 begun = make_int4(0, 0, 0, 0);
-  int64_t at = run.first;
-  int u = run.u, head = run.head;
-  int64_t tile0 = run.tile;
-  Item it{};
-  if (run.left > 0) it = item_of<R, TILE>(p, u);
-  while (run.left > 0) {
-    const int64_t tile1 = min((int64_t)it.tiles, tile0 + run.left);
+  for (Walk<R, TILE, C::OV> w(p, find_run<R, TILE, C::OV, 256>(p, sums, &found)); w.more(); w.next()) {
+    const Item& it = w.it;
+    const int head = w.head;
     // queries: lane (g, t) holds row g of each 8-row tile, at the elements its key chunks cover
     uint32_t qf[NT][HD / 16][2];
     float cq[NT][2];  // score factor and limit of the rows 2t, 2t + 1 of each tile
@@ -336,8 +387,8 @@ __global__ void __launch_bounds__(256, 1) kv_rows_kernel(const __grid_constant__
         for (int i = 0; i < 4; ++i) o[n][j][i] = 0.f;
     }
 
-    const int end = (int)min((int64_t)lim_max, tile1 * TILE);  // positions of this segment
-    int pos = (int)(tile0 * TILE) + warp * STEP;
+    const int end = (int)min((int64_t)lim_max, (int64_t)w.t1 * TILE);  // positions of this segment
+    int pos = w.t0 * TILE + warp * STEP;
     const int32_t* table = p.b.table + it.seq * p.b.max_pages;
     uint32_t kr[MT][2][KCH][4];
     int64_t row = 0;
@@ -554,20 +605,20 @@ __global__ void __launch_bounds__(256, 1) kv_rows_kernel(const __grid_constant__
         }
     }
     __syncthreads();
-    const bool whole = tile0 == 0 && tile1 == it.tiles;
-    float* part = p.part + (int64_t)(2 * blockIdx.x + (tile0 == 0 ? 1 : 0)) * C::kPart;
+    const bool whole = w.whole();
+    float* part = p.part + (int64_t)(2 * blockIdx.x + (w.t0 == 0 ? 1 : 0)) * C::kPart;
     for (int i = tid; i < it.rows * HD; i += 256) {
       const int r = i / HD, d = i % HD;
       float mm = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < C::kWarps; ++w) mm = fmaxf(mm, ml[(w * R + r) * 2]);
+      for (int k = 0; k < C::kWarps; ++k) mm = fmaxf(mm, ml[(k * R + r) * 2]);
       const float base = mm == -INFINITY ? 0.f : mm;
       float acc = 0.f, ll = 0.f;
 #pragma unroll
-      for (int w = 0; w < C::kWarps; ++w) {
-        const float f = ex2(ml[(w * R + r) * 2] - base);
-        acc = fmaf(os[(w * R + r) * HD + d], f, acc);
-        ll = fmaf(ml[(w * R + r) * 2 + 1], f, ll);
+      for (int k = 0; k < C::kWarps; ++k) {
+        const float f = ex2(ml[(k * R + r) * 2] - base);
+        acc = fmaf(os[(k * R + r) * HD + d], f, acc);
+        ll = fmaf(ml[(k * R + r) * 2 + 1], f, ll);
       }
       if (whole) {
         store_out(p, it.q, it.row_lo + r, head, d, HD, ll == 0.f ? 0.f : acc / ll);
@@ -577,17 +628,8 @@ __global__ void __launch_bounds__(256, 1) kv_rows_kernel(const __grid_constant__
         if (d == 0) part[R * HD + 2 * r] = mm, part[R * HD + 2 * r + 1] = ll;
       }
     }
-    if (!whole && tile0 == 0)
-      begun = make_int4(u, head, (int)((at + it.tiles - 1) / run.chunk), 1);
+    if (!whole && w.t0 == 0) begun = w.begun();
     __syncthreads();  // os and ml are free again
-    run.left -= tile1 - tile0;
-    at += tile1 - tile0;
-    tile0 = 0;
-    if (run.left > 0 && ++head == p.pg.n_head_kv) {
-      head = 0;
-      do it = item_of<R, TILE>(p, ++u);
-      while (it.tiles == 0);
-    }
   }
   if (tid == 0) p.desc[blockIdx.x] = begun;
   pdl_trigger();
@@ -610,7 +652,9 @@ template <int HD, int KV>
 struct TileCfg {
   static constexpr int R = 256, TILE = 128;
   static constexpr int ES = KV == KV_E4M3 ? 1 : 2;
-  static constexpr int kThreads = 416, kLoaders = 128;
+  static constexpr int OV = 3;
+  static constexpr int kThreads = 512, kLoaders = 128, kQueryThreads = 96;
+  static constexpr int kSoftmaxRegs = 184, kOtherRegs = 72;  // (184 + 72) * 256 = the 512 * 128 of the launch
   static constexpr int kPlane = 128 * 128;             // 64 elements of 128 rows
   static constexpr int kOperand = HD / 64 * kPlane;    // bytes of a 128-row operand
   static constexpr int kStages = 2;
@@ -619,7 +663,7 @@ struct TileCfg {
 };
 
 struct TileBars {
-  uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], read[4], reset, done;
+  uint64_t q_full, q_empty, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], read[4], reset, done;
 };
 
 // mbar_wait by a whole warp, with one answer: after a timeout no lane goes on alone
@@ -628,38 +672,8 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, uint32
   return __all_sync(0xffffffffu, ok);
 }
 
-// walks a CTA's run, item by item: what every warp role does on its own
-template <int R, int TILE>
-struct Walk {
-  const AttnParams& p;
-  Run run;
-  Item it{};
-  int u, head, seg = 0;
-  int64_t tile0, tile1, at;
-  __device__ Walk(const AttnParams& p_, const Run& r) : p(p_), run(r), u(r.u), head(r.head), tile0(r.tile), tile1(0), at(r.first) {
-    if (run.left > 0) {
-      it = item_of<R, TILE>(p, u);
-      tile1 = min((int64_t)it.tiles, tile0 + run.left);
-    }
-  }
-  __device__ bool more() const { return run.left > 0; }
-  __device__ void next() {
-    run.left -= tile1 - tile0;
-    at += tile1 - tile0;
-    tile0 = 0;
-    ++seg;
-    if (run.left <= 0) return;
-    if (++head == p.pg.n_head_kv) {
-      head = 0;
-      do it = item_of<R, TILE>(p, ++u);
-      while (it.tiles == 0);
-    }
-    tile1 = min((int64_t)it.tiles, run.left);
-  }
-};
-
 template <int HD, int KV>
-__global__ void __launch_bounds__(416, 1) kv_tile_kernel(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(512, 1) kv_tile_kernel(const __grid_constant__ AttnParams p) {
   using C = TileCfg<HD, KV>;
   constexpr bool kBf = KV == KV_BF16;
   constexpr int R = C::R, TILE = C::TILE, ES = C::ES;
@@ -671,6 +685,7 @@ __global__ void __launch_bounds__(416, 1) kv_tile_kernel(const __grid_constant__
   __shared__ Run found;
   __shared__ int not_finite_from[4][HD];  // [item of the run & 3][d]: first position whose value is not finite
   __shared__ int any_not_finite[4];
+  __shared__ float factor_s[2][R];  // [item of the run & 1][row]: what turns a row's products into scores
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* q_s = smem;                                 // [half] operands
   uint8_t* k_s = q_s + 2 * C::kOperand;                // [stage]
@@ -683,7 +698,6 @@ __global__ void __launch_bounds__(416, 1) kv_tile_kernel(const __grid_constant__
   }
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&bar.q_full[i], 128);
       mbar_init(&bar.k_full[i], C::kLoaders);
       mbar_init(&bar.k_empty[i], 1);
       mbar_init(&bar.v_full[i], C::kLoaders);
@@ -694,22 +708,27 @@ __global__ void __launch_bounds__(416, 1) kv_tile_kernel(const __grid_constant__
     }
     for (int i = 0; i < 4; ++i) mbar_init(&bar.read[i], 256);
     mbar_init(&bar.reset, C::kLoaders);
+    mbar_init(&bar.q_full, C::kQueryThreads);
+    mbar_init(&bar.q_empty, 1);
     mbar_init(&bar.done, 1);
     fence_mbar_init();
   }
   if (tid < 4) any_not_finite[tid] = 0;
   tc_fence_before();
-  const Run run = find_run<R, TILE, C::kThreads>(p, sums, &found);  // ends with a barrier of the CTA
+  pdl_wait();
+  const Run run = find_run<R, TILE, C::OV, C::kThreads>(p, sums, &found);  // ends with a barrier of the CTA
   tc_fence_after();
   const uint32_t tmem = tmem_base_s;
   uint32_t* err = p.wait_err;
   constexpr uint32_t kTimeout = DMOE_KV_ERR_TIMEOUT;
-  Walk<R, TILE> w(p, run);
 
+  if (warp >= 8) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
+  Walk<R, TILE, C::OV> w(p, run);
   if (warp == 12) {
     // ---- products
     uint32_t kv_n = 0;           // tiles whose keys were used
-    uint32_t ph_q[2] = {0, 0}, ph_p[2] = {0, 0};
+    uint32_t ph_p[2] = {0, 0};
     bool ok = true;
     const uint32_t k_addr = smem_u32(k_s), v_addr = smem_u32(v_s), q_addr = smem_u32(q_s);
     auto scores = [&](int half, int stage) {
@@ -740,16 +759,14 @@ __global__ void __launch_bounds__(416, 1) kv_tile_kernel(const __grid_constant__
     };
     for (; ok && w.more(); w.next()) {
       const int halves = w.it.rows > 128 ? 2 : 1;
-      const int n = (int)(w.tile1 - w.tile0);
-      for (int h = 0; ok && h < halves; ++h) {
-        ok = warp_wait(&bar.q_full[h], ph_q[h], err, kTimeout);
-        ph_q[h] ^= 1;
-      }
+      const int n = w.t1 - w.t0;
+      ok = warp_wait(&bar.q_full, w.seg & 1, err, kTimeout);
       if (ok) ok = warp_wait(&bar.k_full[kv_n & 1], (kv_n >> 1) & 1, err, kTimeout);
       if (!ok) break;
       tc_fence_after();
       for (int h = 0; h < halves; ++h) scores(h, kv_n & 1);
       commit(&bar.k_empty[kv_n & 1]);
+      if (n == 1) commit(&bar.q_empty);
       for (int j = 0; ok && j < n; ++j, ++kv_n) {
         const int stage = kv_n & 1, next = (kv_n + 1) & 1;
         ok = warp_wait(&bar.v_full[stage], (kv_n >> 1) & 1, err, kTimeout);
@@ -765,7 +782,10 @@ __global__ void __launch_bounds__(416, 1) kv_tile_kernel(const __grid_constant__
             if (!ok) break;
             tc_fence_after();
             scores(h, next);
-            if (h == halves - 1) commit(&bar.k_empty[next]);
+            if (h == halves - 1) {
+              commit(&bar.k_empty[next]);
+              if (j + 2 == n) commit(&bar.q_empty);
+            }
           } else {
             commit(&bar.o_full[h]);
           }
@@ -774,7 +794,72 @@ __global__ void __launch_bounds__(416, 1) kv_tile_kernel(const __grid_constant__
     }
     commit(&bar.done);  // every product that was issued has ended before TMEM is freed
     warp_wait(&bar.done, 0, err, kTimeout);
-  } else if (warp >= 8) {
+  } else if (warp > 12) {
+    // ---- queries: HD / 8 lanes a row, eight rows a lane in flight; rows are scaled into [-1, 1] for f16 products
+    constexpr int LPQ = HD / 8, RPW = 32 / LPQ, DEEP = 6;
+    const int sub = lane % LPQ;
+    for (; w.more(); w.next()) {
+      const Item& it = w.it;
+      const int rows = it.rows > 128 ? 256 : 128;
+      bool first = true, ok = true;
+      for (int r0 = (warp - 13) * RPW; r0 < rows; r0 += 3 * RPW * DEEP) {
+        uint4 x[DEEP];
+#pragma unroll
+        for (int i = 0; i < DEEP; ++i) {
+          const int r = r0 + 3 * RPW * i + lane / LPQ, row = it.row_lo + r;
+          x[i] = make_uint4(0, 0, 0, 0);
+          if (r < it.rows) {
+            const int tok = row / p.group;
+            const uint16_t* s = p.q + (int64_t)(it.q.row0 + tok) * p.q_stride + (int64_t)(w.head * p.group + row - tok * p.group) * HD + 8 * sub;
+            if (p.vec_q16)
+              x[i] = __ldg(reinterpret_cast<const uint4*>(s));
+            else
+              x[i] = make_uint4(s[0] | (uint32_t)s[1] << 16, s[2] | (uint32_t)s[3] << 16, s[4] | (uint32_t)s[5] << 16,
+                                s[6] | (uint32_t)s[7] << 16);
+          }
+        }
+        if (first) {  // the products of the item before have read the operand
+          ok = warp_wait(&bar.q_empty, (w.seg & 1) ^ 1, err, kTimeout);
+          if (!ok) break;
+          first = false;
+        }
+#pragma unroll
+        for (int i = 0; i < DEEP; ++i) {
+          const int r = r0 + 3 * RPW * i + lane / LPQ;
+          uint32_t v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+          float factor = p.scale_log2;
+          if (!(kBf && p.is_bf16)) {
+            float2 f[4];
+            float amax = 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              f[e] = p.is_bf16 ? make_float2(__uint_as_float(v[e] << 16), __uint_as_float(v[e] & 0xffff0000u))
+                               : __half22float2(*reinterpret_cast<const __half2*>(&v[e]));
+              amax = fmaxf(amax, fmaxf(fabsf(f[e].x), fabsf(f[e].y)));
+            }
+            float inv = 1.f;
+            if (!kBf) {
+#pragma unroll
+              for (int o = LPQ / 2; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+              const int e = min(max((int)(__float_as_uint(amax) >> 23) - 126, -100), 100);
+              inv = pow2i(-e);
+              factor *= pow2i(e);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = pack2<kBf>(f[e].x * inv, f[e].y * inv);
+          }
+          if (r < rows) {
+            *reinterpret_cast<uint4*>(q_s + (r / 128) * C::kOperand + (sub / 8) * C::kPlane + (r % 128) * 128 + 16 * ((sub % 8) ^ (r & 7))) =
+                make_uint4(v[0], v[1], v[2], v[3]);
+            if (sub == 0) factor_s[w.seg & 1][r] = factor;
+          }
+        }
+      }
+      if (!ok) break;
+      fence_proxy_async_smem();
+      mbar_arrive(&bar.q_full);
+    }
+  } else {
     // ---- keys and values
     const int lt = tid - 256;
     constexpr int LPR = HD * ES / 16;             // lanes a row, 16 bytes each
@@ -827,16 +912,15 @@ __global__ void __launch_bounds__(416, 1) kv_tile_kernel(const __grid_constant__
       return warp_wait(&bar.reset, seg & 1, err, kTimeout);
     };
     if constexpr (KV == KV_E4M3) {
-      uint4 kr[N], vr[N];
-      auto fetch = [&](uint4 (&x)[N], const void* base, int tile, int lim) {
+      uint4 x[N];  // the tile's keys, then its values, then the next tile's keys: one of them is on its way
+      auto fetch = [&](const void* base, int tile, int lim) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-          const int r = r0 + i * RPI;
           x[i] = make_uint4(0, 0, 0, 0);
-          if (tile * TILE + r < lim) x[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(base) + source(i)));
+          if (tile * TILE + r0 + i * RPI < lim) x[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(base) + source(i)));
         }
       };
-      auto put = [&](const uint4 (&x)[N], uint8_t* dst) {
+      auto put = [&](uint8_t* dst) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
           const int r = r0 + i * RPI;
@@ -854,35 +938,23 @@ __global__ void __launch_bounds__(416, 1) kv_tile_kernel(const __grid_constant__
       };
       if (w.more()) {
         const int lim = row_limit(p, w.it.q, w.it.row_lo + w.it.rows - 1);
-        get_pages(w.it, w.head, (int)w.tile0, lim, true);
-        fetch(kr, p.pg.k, (int)w.tile0, lim);
-        fetch(vr, p.pg.v, (int)w.tile0, lim);
+        get_pages(w.it, w.head, w.t0, lim, true);
+        fetch(p.pg.k, w.t0, lim);
       }
       while (ok && w.more()) {
         const int lim_min = row_limit(p, w.it.q, w.it.row_lo);
         const int lim_max = row_limit(p, w.it.q, w.it.row_lo + w.it.rows - 1);
-        const int seg = w.seg, head = w.head;
-        const Item it = w.it;
-        const int t0 = (int)w.tile0, t1 = (int)w.tile1;
-        w.next();
+        const int seg = w.seg;
+        const int t0 = w.t0, t1 = w.t1;
         for (int t = t0; t < t1; ++t, ++kv_n) {
           const int stage = kv_n & 1;
           const uint32_t ph = ((kv_n >> 1) & 1) ^ 1;
           ok = warp_wait(&bar.k_empty[stage], ph, err, kTimeout);
           if (!ok) break;
-          put(kr, k_s + stage * C::kOperand);
+          put(k_s + stage * C::kOperand);
           fence_proxy_async_smem();
           mbar_arrive(&bar.k_full[stage]);
-          // the next tile of this item or of the next one
-          const bool same = t + 1 < t1, more = same || w.more();
-          const Item& ni = same ? it : w.it;
-          const int nh = same ? head : w.head;
-          const int nt = same ? t + 1 : (int)w.tile0;
-          const int nl = same ? lim_max : more ? row_limit(p, w.it.q, w.it.row_lo + w.it.rows - 1) : 0;
-          if (more) {
-            get_pages(ni, nh, nt, nl, !same);
-            fetch(kr, p.pg.k, nt, nl);
-          }
+          fetch(p.pg.v, t, lim_max);
           ok = warp_wait(&bar.v_empty[stage], ph, err, kTimeout);
           if (!ok) break;
           if (t == t0 && !reset_marks(seg)) {
@@ -893,7 +965,7 @@ __global__ void __launch_bounds__(416, 1) kv_tile_kernel(const __grid_constant__
 #pragma unroll
             for (int i = 0; i < N; ++i) {
               const int pos = t * TILE + r0 + i * RPI;
-              uint32_t v[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
+              uint32_t v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 const uint32_t bad = __vcmpeq4(v[e] & 0x7f7f7f7fu, 0x7f7f7f7fu);
@@ -903,13 +975,21 @@ __global__ void __launch_bounds__(416, 1) kv_tile_kernel(const __grid_constant__
                   v[e] &= ~bad;
                 }
               }
-              vr[i] = make_uint4(v[0], v[1], v[2], v[3]);
+              x[i] = make_uint4(v[0], v[1], v[2], v[3]);
             }
           }
-          put(vr, v_s + stage * C::kOperand);
+          put(v_s + stage * C::kOperand);
           fence_proxy_async_smem();
           mbar_arrive(&bar.v_full[stage]);
-          if (more) fetch(vr, p.pg.v, nt, nl);
+          // the keys of the next tile of this item, or of the next item's first
+          const bool same = t + 1 < t1;
+          if (!same) w.next();
+          if (same || w.more()) {
+            const int nt = same ? t + 1 : w.t0;
+            const int lim = same ? lim_max : row_limit(p, w.it.q, w.it.row_lo + w.it.rows - 1);
+            get_pages(w.it, w.head, nt, lim, !same);
+            fetch(p.pg.k, nt, lim);
+          }
         }
       }
     } else {
@@ -927,27 +1007,25 @@ __global__ void __launch_bounds__(416, 1) kv_tile_kernel(const __grid_constant__
       };
       if (w.more()) {
         const int lim = row_limit(p, w.it.q, w.it.row_lo + w.it.rows - 1);
-        get_pages(w.it, w.head, (int)w.tile0, lim, true);
-        issue(p.pg.k, k_s, (int)w.tile0, lim);  // the ring is empty
-        issue(p.pg.v, v_s, (int)w.tile0, lim);
+        get_pages(w.it, w.head, w.t0, lim, true);
+        issue(p.pg.k, k_s, w.t0, lim);  // the ring is empty
+        issue(p.pg.v, v_s, w.t0, lim);
       }
       while (ok && w.more()) {
         const int lim_min = row_limit(p, w.it.q, w.it.row_lo);
         const int lim_max = row_limit(p, w.it.q, w.it.row_lo + w.it.rows - 1);
-        const int seg = w.seg, head = w.head;
-        const Item it = w.it;
-        const int t0 = (int)w.tile0, t1 = (int)w.tile1;
-        w.next();
+        const int seg = w.seg;
+        const int t0 = w.t0, t1 = w.t1;
         for (int t = t0; t < t1; ++t, ++kv_n) {
           const int stage = kv_n & 1, next = (kv_n + 1) & 1;
           const uint32_t ph = (((kv_n + 1) >> 1) & 1) ^ 1;
-          const bool same = t + 1 < t1, more = same || w.more();
-          const Item& ni = same ? it : w.it;
-          const int nh = same ? head : w.head;
-          const int nt = same ? t + 1 : (int)w.tile0;
+          const bool same = t + 1 < t1;
+          if (!same) w.next();  // this tile's item is left: only its limits are used below
+          const bool more = same || w.more();
+          const int nt = same ? t + 1 : w.t0;
           const int nl = same ? lim_max : more ? row_limit(p, w.it.q, w.it.row_lo + w.it.rows - 1) : 0;
           if (more) {
-            get_pages(ni, nh, nt, nl, !same);
+            get_pages(w.it, w.head, nt, nl, !same);
             ok = warp_wait(&bar.k_empty[next], ph, err, kTimeout);
             if (!ok) break;
             issue(p.pg.k, k_s + next * C::kOperand, nt, nl);
@@ -993,8 +1071,11 @@ __global__ void __launch_bounds__(416, 1) kv_tile_kernel(const __grid_constant__
       }
       asm volatile("cp.async.wait_all;" ::: "memory");
     }
+  }
   } else {
     // ---- softmax of one half
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kSoftmaxRegs));
+    Walk<R, TILE, C::OV> w(p, run);
     const int half = warp >> 2, quarter = warp & 3;
     const int my = half * 128 + quarter * 32 + lane;  // row of the item
     const uint32_t s_addr = tmem_addr(tmem, quarter * 32, half * 128), o_addr = tmem_addr(tmem, quarter * 32, 256 + half * 128);
@@ -1003,71 +1084,19 @@ __global__ void __launch_bounds__(416, 1) kv_tile_kernel(const __grid_constant__
     int4 begun = make_int4(0, 0, 0, 0);
     for (; ok && w.more(); w.next()) {
       const Item& it = w.it;
-      const bool whole = w.tile0 == 0 && w.tile1 == it.tiles;
-      if (!whole && w.tile0 == 0) begun = make_int4(w.u, w.head, (int)((w.at + it.tiles - 1) / run.chunk), 1);
+      const bool whole = w.whole();
+      if (!whole && w.t0 == 0) begun = w.begun();
       if (half * 128 >= it.rows) {
         mbar_arrive(&bar.read[w.seg & 3]);
         continue;
       }
       const bool live = my < it.rows;
       const int row = it.row_lo + my;
-      // the row's queries into the operand, scaled into [-1, 1] for f16 products
-      float factor = p.scale_log2;
-      {
-        uint32_t x[HD / 2];
-        const int64_t at = (int64_t)(it.q.row0 + row / p.group) * p.q_stride + (int64_t)(w.head * p.group + row % p.group) * HD;
-#pragma unroll
-        for (int i = 0; i < HD / 8; ++i) {
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (live) {
-            if (p.vec_q16) {
-              v = __ldg(reinterpret_cast<const uint4*>(p.q + at) + i);
-            } else {
-              const uint16_t* s = p.q + at + 8 * i;
-              v = make_uint4(s[0] | (uint32_t)s[1] << 16, s[2] | (uint32_t)s[3] << 16, s[4] | (uint32_t)s[5] << 16,
-                             s[6] | (uint32_t)s[7] << 16);
-            }
-          }
-          x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
-        }
-        auto value = [&](uint32_t v) {
-          if (p.is_bf16) return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
-          return __half22float2(*reinterpret_cast<const __half2*>(&v));
-        };
-        if (!(kBf && p.is_bf16)) {
-          float inv = 1.f;
-          if (!kBf) {
-            float amax = 0.f;
-#pragma unroll
-            for (int i = 0; i < HD / 2; ++i) {
-              const float2 f = value(x[i]);
-              amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
-            }
-            const int e = min(max((int)(__float_as_uint(amax) >> 23) - 126, -100), 100);
-            inv = pow2i(-e);
-            factor *= pow2i(e);
-          }
-#pragma unroll
-          for (int i = 0; i < HD / 2; ++i) {
-            const float2 f = value(x[i]);
-            x[i] = pack2<kBf>(f.x * inv, f.y * inv);
-          }
-        }
-        const int r = quarter * 32 + lane;
-        uint8_t* dst = q_s + half * C::kOperand + r * 128;
-#pragma unroll
-        for (int i = 0; i < HD / 8; ++i)
-          *reinterpret_cast<uint4*>(dst + (i / 8) * C::kPlane + 16 * ((i % 8) ^ (r & 7))) =
-              make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
-      }
-      fence_proxy_async_smem();
-      mbar_arrive(&bar.q_full[half]);
       const int lim_all = row_limit(p, it.q, it.row_lo + it.rows - 1);
       const int lim = live ? row_limit(p, it.q, row) : lim_all;
       const int lim_warp = row_limit(p, it.q, it.row_lo + min(it.rows - 1, half * 128 + quarter * 32));
       float m = -INFINITY, l = 0.f;  // reference of the weights, sum
-      // scale exponents of a tile's four 32-position blocks: lanes 0-3
-      int sc = 0, sc_next = 0;
+      // scale exponents of a tile's four 32-position blocks: lanes 0-3, a tile ahead
       auto get_scales = [&](int tile) {
         int e = 127 | 127 << 8;
         const uint32_t b = tile * (TILE / 32) + (lane & 3);
@@ -1080,11 +1109,13 @@ __global__ void __launch_bounds__(416, 1) kv_tile_kernel(const __grid_constant__
         }
         return e;
       };
-      const int t0 = (int)w.tile0, t1 = (int)w.tile1;
-      sc_next = get_scales(t0);
-      for (int t = t0; t < t1; ++t) {
-        sc = sc_next;
-        if (t + 1 < t1) sc_next = get_scales(t + 1);
+      int sc_next = get_scales(w.t0);
+      ok = warp_wait(&bar.q_full, w.seg & 1, err, kTimeout);
+      if (!ok) break;
+      const float factor = factor_s[w.seg & 1][my];
+      for (int t = w.t0; t < w.t1; ++t) {
+        const int sc = sc_next;
+        if (t + 1 < w.t1) sc_next = get_scales(t + 1);
         float c[4], ev[4];
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
@@ -1096,23 +1127,27 @@ __global__ void __launch_bounds__(416, 1) kv_tile_kernel(const __grid_constant__
         if (!ok) break;
         ph_s ^= 1;
         tc_fence_after();
-        const int valid = min(TILE, max(0, lim - t * TILE));  // columns this row sees
-        const bool edge = (t + 1) * TILE > lim_warp;
+        uint32_t x[4][32];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) tmem_ld32(s_addr + 32 * b, x[b]);
+        tmem_wait_ld();
+        if ((t + 1) * TILE > lim_warp) {
+          const int valid = lim - t * TILE;  // columns this row sees
+#pragma unroll
+          for (int b = 0; b < 4; ++b)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (32 * b + i >= valid) x[b][i] = 0xff800000u;
+        }
         float mx = -INFINITY;
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-          uint32_t x[32];
-          tmem_ld32(s_addr + 32 * b, x);
-          tmem_wait_ld();
-          float top = -INFINITY;
-          if (edge) {
+          float top[4];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) top = fmaxf(top, 32 * b + i < valid ? __uint_as_float(x[i]) : -INFINITY);
-          } else {
+          for (int i = 0; i < 4; ++i) top[i] = __uint_as_float(x[b][i]);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) top = fmaxf(top, __uint_as_float(x[i]));
-          }
-          mx = fmaxf(mx, fmaf(top, c[b], ev[b]));
+          for (int i = 4; i < 32; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(x[b][i]));
+          mx = fmaxf(mx, fmaf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), c[b], ev[b]));
         }
         float shrink = 1.f;
         if (mx > m + 8.f || m == -INFINITY) {
@@ -1121,40 +1156,32 @@ __global__ void __launch_bounds__(416, 1) kv_tile_kernel(const __grid_constant__
           m = to;
           l *= shrink;
         }
-        if (t > t0 && __any_sync(0xffffffffu, shrink != 1.f)) {
+        if (t > w.t0 && __any_sync(0xffffffffu, shrink != 1.f)) {
           // the products of the tile before have ended: the scores' arrival counts them
 #pragma unroll 1
           for (int d = 0; d < HD; d += 16) {
-            uint32_t x[16];
-            tmem_ld16(o_addr + d, x);
+            uint32_t y[16];
+            tmem_ld16(o_addr + d, y);
             tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * shrink);
-            tmem_st16(o_addr + d, x);
+            for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * shrink);
+            tmem_st16(o_addr + d, y);
           }
         }
         const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-          uint32_t x[32];
-          tmem_ld32(s_addr + 32 * b, x);
-          tmem_wait_ld();
           const float off = ev[b] - base;
-          float sum = 0.f;
+          float sum[2] = {0.f, 0.f};
           uint32_t pk[16];
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
-            float a = fmaf(__uint_as_float(x[i]), c[b], off), d = fmaf(__uint_as_float(x[i + 1]), c[b], off);
-            if (edge) {
-              a = 32 * b + i < valid ? a : -INFINITY;
-              d = 32 * b + i + 1 < valid ? d : -INFINITY;
-            }
-            a = ex2(a), d = ex2(d);
-            sum += a + d;
+            const float a = ex2(fmaf(__uint_as_float(x[b][i]), c[b], off)), d = ex2(fmaf(__uint_as_float(x[b][i + 1]), c[b], off));
+            sum[0] += a, sum[1] += d;
             pk[i / 2] = pack2<kBf>(a, d);
           }
-          l = fmaf(sum, KV == KV_E4M3 ? pow2i(-(int)ev[b]) : 1.f, l);
           tmem_st16(s_addr + 16 * b, pk);
+          l = fmaf(sum[0] + sum[1], KV == KV_E4M3 ? pow2i(-(int)ev[b]) : 1.f, l);
         }
         tmem_wait_st();
         tc_fence_before();
@@ -1166,38 +1193,45 @@ __global__ void __launch_bounds__(416, 1) kv_tile_kernel(const __grid_constant__
       ph_o ^= 1;
       tc_fence_after();
       const bool marked = *const_cast<volatile int*>(&any_not_finite[w.seg & 3]) != 0;
-      float* part = p.part + (int64_t)(2 * blockIdx.x + (w.tile0 == 0 ? 1 : 0)) * C::kPart;
+      float* part = p.part + (int64_t)(2 * blockIdx.x + (w.t0 == 0 ? 1 : 0)) * C::kPart;
       const float inv = l == 0.f ? 0.f : 1.f / l;
       const int64_t at = (int64_t)(it.q.row0 + row / p.group) * p.out_stride + (int64_t)(w.head * p.group + row % p.group) * HD;
-#pragma unroll 1
-      for (int d = 0; d < HD; d += 16) {
-        uint32_t x[16];
-        tmem_ld16(o_addr + d, x);
+#pragma unroll
+      for (int d0 = 0; d0 < HD; d0 += 64) {
+        uint32_t x[64];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) tmem_ld32(o_addr + d0 + 32 * i, reinterpret_cast<uint32_t(&)[32]>(x[32 * i]));
         tmem_wait_ld();
         if (marked) {
+#pragma unroll 1
+          for (int i = 0; i < 64; ++i)
+            if (*const_cast<volatile int*>(&not_finite_from[w.seg & 3][d0 + i]) < lim) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (*const_cast<volatile int*>(&not_finite_from[w.seg & 3][d + i]) < lim) x[i] = 0x7fc00000u;
+              for (int e = 0; e < 64; ++e)
+                if (e == i) x[e] = 0x7fc00000u;
+            }
         }
         if (!live) continue;
         if (whole) {
-          uint32_t h[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float a = l == 0.f ? 0.f : __uint_as_float(x[2 * i]) * inv, b = l == 0.f ? 0.f : __uint_as_float(x[2 * i + 1]) * inv;
-            h[i] = p.is_bf16 ? pack2<true>(a, b) : pack2<false>(a, b);
-          }
-          if (p.vec_out16) {
-            reinterpret_cast<uint4*>(p.out + at + d)[0] = make_uint4(h[0], h[1], h[2], h[3]);
-            reinterpret_cast<uint4*>(p.out + at + d)[1] = make_uint4(h[4], h[5], h[6], h[7]);
-          } else {
+          for (int i = 0; i < 64; i += 8) {
+            uint32_t h[4];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) p.out[at + d + i] = (uint16_t)(h[i / 2] >> (16 * (i & 1)));
+            for (int e = 0; e < 4; ++e) {
+              const float a = l == 0.f ? 0.f : __uint_as_float(x[i + 2 * e]) * inv, b = l == 0.f ? 0.f : __uint_as_float(x[i + 2 * e + 1]) * inv;
+              h[e] = p.is_bf16 ? pack2<true>(a, b) : pack2<false>(a, b);
+            }
+            if (p.vec_out16) {
+              *reinterpret_cast<uint4*>(p.out + at + d0 + i) = make_uint4(h[0], h[1], h[2], h[3]);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) p.out[at + d0 + i + e] = (uint16_t)(h[e / 2] >> (16 * (e & 1)));
+            }
           }
         } else {
-          float4* to = reinterpret_cast<float4*>(part + my * HD + d);
+          float4* to = reinterpret_cast<float4*>(part + my * HD + d0);
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
+          for (int i = 0; i < 16; ++i)
             to[i] = make_float4(__uint_as_float(x[4 * i]), __uint_as_float(x[4 * i + 1]), __uint_as_float(x[4 * i + 2]),
                                 __uint_as_float(x[4 * i + 3]));
         }
@@ -1285,10 +1319,9 @@ cudaError_t launch_rows(AttnParams p, int max_rows, cudaStream_t st) {
   static_assert(C::kSmem <= 227 * 1024, "shared memory");
   cudaError_t e = cudaFuncSetAttribute(kv_rows_kernel<HD, KV, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmem);
   if (e != cudaSuccess) return e;
-  kv_rows_kernel<HD, KV, NT><<<kRowsGrid, 256, C::kSmem, st>>>(p);
-  e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
   set_pdl_for_call(true);
+  e = launch_pdl(kv_rows_kernel<HD, KV, NT>, dim3(kRowsGrid), dim3(256), C::kSmem, st, p);
+  if (e != cudaSuccess) return e;
   e = launch_pdl(kv_combine_kernel<HD, C::R, C::TILE, 8>, dim3(kRowsGrid, C::R), dim3(8 * HD / 4), 0, st, p);
   set_pdl_for_call(false);
   return e;
@@ -1301,10 +1334,9 @@ cudaError_t launch_tiles(AttnParams p, int max_rows, cudaStream_t st) {
   static_assert(C::kSmem <= 220 * 1024, "shared memory");
   cudaError_t e = cudaFuncSetAttribute(kv_tile_kernel<HD, KV>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmem);
   if (e != cudaSuccess) return e;
-  kv_tile_kernel<HD, KV><<<kTileGrid, C::kThreads, C::kSmem, st>>>(p);
-  e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
   set_pdl_for_call(true);
+  e = launch_pdl(kv_tile_kernel<HD, KV>, dim3(kTileGrid), dim3(C::kThreads), C::kSmem, st, p);
+  if (e != cudaSuccess) return e;
   e = launch_pdl(kv_combine_kernel<HD, C::R, C::TILE, 1>, dim3(kTileGrid, C::R / 8), dim3(8 * HD / 4), 0, st, p);
   set_pdl_for_call(false);
   return e;
