@@ -41,6 +41,7 @@ struct AttnParams {
   int64_t q_stride, out_stride;
   int is_bf16;       // type of q and out
   int n_head, group;
+  uint32_t group_magic;  // ceil(2^28 / group): x / group for x < 2^13 and group <= 2^12 (x * error < 2^28)
   int block_length;
   int n_qt;          // row tiles a sequence can have (max_q_len)
   int vec_q, vec_q16, vec_out16;  // q rows allow 8-byte, 16-byte loads; out rows 16-byte stores
@@ -54,6 +55,30 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// two floats as one 64-bit operand of the packed fma and add
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
 }
 
 // 2^e for |e| <= 126
@@ -652,9 +677,10 @@ template <int HD, int KV>
 struct TileCfg {
   static constexpr int R = 256, TILE = 128;
   static constexpr int ES = KV == KV_E4M3 ? 1 : 2;
-  static constexpr int OV = 3;
-  static constexpr int kThreads = 512, kLoaders = 128, kQueryThreads = 96;
-  static constexpr int kSoftmaxRegs = 184, kOtherRegs = 72;  // (184 + 72) * 256 = the 512 * 128 of the launch
+  static constexpr int OV = 2;
+  static constexpr int kThreads = 640, kLoaders = 128;
+  // registers a thread: 256 * 160 + 256 * 64 + 128 * 32 = the 640 * 96 of the launch
+  static constexpr int kSoftmaxRegs = 160, kLoadRegs = 64, kIssueRegs = 32;
   static constexpr int kPlane = 128 * 128;             // 64 elements of 128 rows
   static constexpr int kOperand = HD / 64 * kPlane;    // bytes of a 128-row operand
   static constexpr int kStages = 2;
@@ -663,7 +689,7 @@ struct TileCfg {
 };
 
 struct TileBars {
-  uint64_t q_full, q_empty, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], read[4], reset, done;
+  uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], read[4], reset, done;
 };
 
 // mbar_wait by a whole warp, with one answer: after a timeout no lane goes on alone
@@ -673,7 +699,7 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, uint32
 }
 
 template <int HD, int KV>
-__global__ void __launch_bounds__(512, 1) kv_tile_kernel(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__ AttnParams p) {
   using C = TileCfg<HD, KV>;
   constexpr bool kBf = KV == KV_BF16;
   constexpr int R = C::R, TILE = C::TILE, ES = C::ES;
@@ -685,14 +711,13 @@ __global__ void __launch_bounds__(512, 1) kv_tile_kernel(const __grid_constant__
   __shared__ Run found;
   __shared__ int not_finite_from[4][HD];  // [item of the run & 3][d]: first position whose value is not finite
   __shared__ int any_not_finite[4];
-  __shared__ float factor_s[2][R];  // [item of the run & 1][row]: what turns a row's products into scores
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* q_s = smem;                                 // [half] operands
   uint8_t* k_s = q_s + 2 * C::kOperand;                // [stage]
   uint8_t* v_s = k_s + C::kStages * C::kOperand;       // [stage]
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
-  if (warp == 12) {
+  if (warp == 16) {
     tmem_alloc(&tmem_base_s, 512);
     tmem_relinquish();
   }
@@ -708,8 +733,7 @@ __global__ void __launch_bounds__(512, 1) kv_tile_kernel(const __grid_constant__
     }
     for (int i = 0; i < 4; ++i) mbar_init(&bar.read[i], 256);
     mbar_init(&bar.reset, C::kLoaders);
-    mbar_init(&bar.q_full, C::kQueryThreads);
-    mbar_init(&bar.q_empty, 1);
+    mbar_init(&bar.q_full, 256);
     mbar_init(&bar.done, 1);
     fence_mbar_init();
   }
@@ -722,10 +746,10 @@ __global__ void __launch_bounds__(512, 1) kv_tile_kernel(const __grid_constant__
   uint32_t* err = p.wait_err;
   constexpr uint32_t kTimeout = DMOE_KV_ERR_TIMEOUT;
 
-  if (warp >= 8) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
-  Walk<R, TILE, C::OV> w(p, run);
-  if (warp == 12) {
+  if (warp >= 16) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kIssueRegs));
+    Walk<R, TILE, C::OV> w(p, run);
+    if (warp == 16) {
     // ---- products
     uint32_t kv_n = 0;           // tiles whose keys were used
     uint32_t ph_p[2] = {0, 0};
@@ -766,7 +790,6 @@ __global__ void __launch_bounds__(512, 1) kv_tile_kernel(const __grid_constant__
       tc_fence_after();
       for (int h = 0; h < halves; ++h) scores(h, kv_n & 1);
       commit(&bar.k_empty[kv_n & 1]);
-      if (n == 1) commit(&bar.q_empty);
       for (int j = 0; ok && j < n; ++j, ++kv_n) {
         const int stage = kv_n & 1, next = (kv_n + 1) & 1;
         ok = warp_wait(&bar.v_full[stage], (kv_n >> 1) & 1, err, kTimeout);
@@ -782,10 +805,7 @@ __global__ void __launch_bounds__(512, 1) kv_tile_kernel(const __grid_constant__
             if (!ok) break;
             tc_fence_after();
             scores(h, next);
-            if (h == halves - 1) {
-              commit(&bar.k_empty[next]);
-              if (j + 2 == n) commit(&bar.q_empty);
-            }
+            if (h == halves - 1) commit(&bar.k_empty[next]);
           } else {
             commit(&bar.o_full[h]);
           }
@@ -794,91 +814,33 @@ __global__ void __launch_bounds__(512, 1) kv_tile_kernel(const __grid_constant__
     }
     commit(&bar.done);  // every product that was issued has ended before TMEM is freed
     warp_wait(&bar.done, 0, err, kTimeout);
-  } else if (warp > 12) {
-    // ---- queries: HD / 8 lanes a row, eight rows a lane in flight; rows are scaled into [-1, 1] for f16 products
-    constexpr int LPQ = HD / 8, RPW = 32 / LPQ, DEEP = 6;
-    const int sub = lane % LPQ;
-    for (; w.more(); w.next()) {
-      const Item& it = w.it;
-      const int rows = it.rows > 128 ? 256 : 128;
-      bool first = true, ok = true;
-      for (int r0 = (warp - 13) * RPW; r0 < rows; r0 += 3 * RPW * DEEP) {
-        uint4 x[DEEP];
-#pragma unroll
-        for (int i = 0; i < DEEP; ++i) {
-          const int r = r0 + 3 * RPW * i + lane / LPQ, row = it.row_lo + r;
-          x[i] = make_uint4(0, 0, 0, 0);
-          if (r < it.rows) {
-            const int tok = row / p.group;
-            const uint16_t* s = p.q + (int64_t)(it.q.row0 + tok) * p.q_stride + (int64_t)(w.head * p.group + row - tok * p.group) * HD + 8 * sub;
-            if (p.vec_q16)
-              x[i] = __ldg(reinterpret_cast<const uint4*>(s));
-            else
-              x[i] = make_uint4(s[0] | (uint32_t)s[1] << 16, s[2] | (uint32_t)s[3] << 16, s[4] | (uint32_t)s[5] << 16,
-                                s[6] | (uint32_t)s[7] << 16);
-          }
-        }
-        if (first) {  // the products of the item before have read the operand
-          ok = warp_wait(&bar.q_empty, (w.seg & 1) ^ 1, err, kTimeout);
-          if (!ok) break;
-          first = false;
-        }
-#pragma unroll
-        for (int i = 0; i < DEEP; ++i) {
-          const int r = r0 + 3 * RPW * i + lane / LPQ;
-          uint32_t v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-          float factor = p.scale_log2;
-          if (!(kBf && p.is_bf16)) {
-            float2 f[4];
-            float amax = 0.f;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              f[e] = p.is_bf16 ? make_float2(__uint_as_float(v[e] << 16), __uint_as_float(v[e] & 0xffff0000u))
-                               : __half22float2(*reinterpret_cast<const __half2*>(&v[e]));
-              amax = fmaxf(amax, fmaxf(fabsf(f[e].x), fabsf(f[e].y)));
-            }
-            float inv = 1.f;
-            if (!kBf) {
-#pragma unroll
-              for (int o = LPQ / 2; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-              const int e = min(max((int)(__float_as_uint(amax) >> 23) - 126, -100), 100);
-              inv = pow2i(-e);
-              factor *= pow2i(e);
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = pack2<kBf>(f[e].x * inv, f[e].y * inv);
-          }
-          if (r < rows) {
-            *reinterpret_cast<uint4*>(q_s + (r / 128) * C::kOperand + (sub / 8) * C::kPlane + (r % 128) * 128 + 16 * ((sub % 8) ^ (r & 7))) =
-                make_uint4(v[0], v[1], v[2], v[3]);
-            if (sub == 0) factor_s[w.seg & 1][r] = factor;
-          }
-        }
-      }
-      if (!ok) break;
-      fence_proxy_async_smem();
-      mbar_arrive(&bar.q_full);
     }
-  } else {
-    // ---- keys and values
-    const int lt = tid - 256;
+  } else if (warp >= 8) {
+    // ---- keys (warps 8-11) and values (12-15)
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kLoadRegs));
+    Walk<R, TILE, C::OV> w(p, run);
+    const bool is_v = warp >= 12;
+    const int lt = tid & 127;
+    uint64_t* const full = is_v ? bar.v_full : bar.k_full;
+    uint64_t* const empty = is_v ? bar.v_empty : bar.k_empty;
+    uint8_t* const ring = is_v ? v_s : k_s;
+    const uint8_t* const base = static_cast<const uint8_t*>(is_v ? p.pg.v : p.pg.k);
     constexpr int LPR = HD * ES / 16;             // lanes a row, 16 bytes each
     constexpr int RPI = C::kLoaders / LPR;        // rows an instruction of all loaders covers
     constexpr int N = TILE / RPI;                 // 16-byte pieces a thread loads of a tile
     const int c = lt % LPR, r0 = lt / LPR;
-    uint32_t kv_n = 0;
     bool ok = true;
     // first row of each of the tile's 32-position blocks in the pages. The page numbers of eight tiles
     // are read at once, one a lane
     int64_t first_row[4];
-    int held = 0, held_from = 0, held_to = 0;  // blocks [held_from, held_to) of the item
-    auto get_pages = [&](const Item& it, int head, int tile, int lim, bool new_item) {
+    int held = 0, held_from = 0;  // blocks [held_from, held_from + 32) of the item
+    auto get_pages = [&](int tile, int lim, bool new_item) {
       const int b0 = tile * (TILE / 32);
-      if (new_item || b0 >= held_to) {
-        held_from = b0, held_to = b0 + 32;
+      if (new_item || b0 >= held_from + 32) {
+        held_from = b0;
         held = 0;
         if ((b0 + lane) * 32 < lim) {
-          held = p.b.table[it.seq * p.b.max_pages + kv_slot(p.pg, b0 + lane)];
+          held = p.b.table[w.it.seq * p.b.max_pages + kv_slot(p.pg, b0 + lane)];
           if (held < 0 || held >= p.pg.n_pages) {
             kv_report(p.pg.err, DMOE_KV_ERR_PAGE);
             held = 0;
@@ -889,16 +851,13 @@ __global__ void __launch_bounds__(512, 1) kv_tile_kernel(const __grid_constant__
       for (int i = 0; i < 4; ++i) {
         const int page = __shfl_sync(0xffffffffu, held, b0 + i - held_from);
         const uint32_t b = b0 + i;
-        first_row[i] = kv_row(p.pg, page, head, (int)(b - kv_slot(p.pg, b) * p.pg.page_blocks) * kScaleBlock);
+        first_row[i] = kv_row(p.pg, page, w.head, (int)(b - kv_slot(p.pg, b) * p.pg.page_blocks) * kScaleBlock);
       }
     };
-    // byte offset of this thread's i-th piece of the tile; its row is r0 + i * RPI
-    auto source = [&](int i) {
-      const int r = r0 + i * RPI;
-      return (first_row[i * RPI / 32] + (r & 31)) * (HD * ES) + 16 * c;
-    };
-    // positions that only some rows see, and values that are not finite there: their products with a zero
-    // weight would reach the others. They are set to zero, and their element marked for the rows that see them
+    // this thread's i-th piece of the tile; its row is r0 + i * RPI
+    auto source = [&](int i) { return base + (first_row[i * RPI / 32] + ((r0 + i * RPI) & 31)) * (HD * ES) + 16 * c; };
+    // Values at positions that only some rows see, where they are not finite: their products with a zero
+    // weight would reach the other rows. They are set to zero, and their element marked for the rows that see them
     auto mark = [&](int seg, int pos, int d) {
       atomicMin(&not_finite_from[seg & 3][d], pos);
       any_not_finite[seg & 3] = 1;
@@ -911,57 +870,35 @@ __global__ void __launch_bounds__(512, 1) kv_tile_kernel(const __grid_constant__
       mbar_arrive(&bar.reset);
       return warp_wait(&bar.reset, seg & 1, err, kTimeout);
     };
-    if constexpr (KV == KV_E4M3) {
-      uint4 x[N];  // the tile's keys, then its values, then the next tile's keys: one of them is on its way
-      auto fetch = [&](const void* base, int tile, int lim) {
+    auto limit = [&]() { return row_limit(p, w.it.q, w.it.row_lo + w.it.rows - 1); };
+    uint4 x[KV == KV_E4M3 ? N : 1];  // 8-bit pages: the next tile, on its way
+    auto fetch = [&](int tile, int lim) {
+      if constexpr (KV == KV_E4M3) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
           x[i] = make_uint4(0, 0, 0, 0);
-          if (tile * TILE + r0 + i * RPI < lim) x[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(base) + source(i)));
+          if (tile * TILE + r0 + i * RPI < lim) x[i] = __ldg(reinterpret_cast<const uint4*>(source(i)));
         }
-      };
-      auto put = [&](uint8_t* dst) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const int r = r0 + i * RPI;
-          const uint32_t v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-          uint32_t h[8];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) h[2 * e] = e4m3_pair<0>(v[e]), h[2 * e + 1] = e4m3_pair<1>(v[e]);
-          const uint4 a = make_uint4(h[0], h[1], h[2], h[3]), b = make_uint4(h[4], h[5], h[6], h[7]);
-          uint8_t* row = dst + (c / 4) * C::kPlane + r * 128;
-          const int first = (c / 4) & 1;  // lanes of the two planes take turns: no bank twice
-          const int ca = (2 * (c % 4)) ^ (r & 7), cb = (2 * (c % 4) + 1) ^ (r & 7);
-          *reinterpret_cast<uint4*>(row + 16 * (first ? cb : ca)) = first ? b : a;
-          *reinterpret_cast<uint4*>(row + 16 * (first ? ca : cb)) = first ? a : b;
-        }
-      };
-      if (w.more()) {
-        const int lim = row_limit(p, w.it.q, w.it.row_lo + w.it.rows - 1);
-        get_pages(w.it, w.head, w.t0, lim, true);
-        fetch(p.pg.k, w.t0, lim);
       }
-      while (ok && w.more()) {
-        const int lim_min = row_limit(p, w.it.q, w.it.row_lo);
-        const int lim_max = row_limit(p, w.it.q, w.it.row_lo + w.it.rows - 1);
-        const int seg = w.seg;
-        const int t0 = w.t0, t1 = w.t1;
-        for (int t = t0; t < t1; ++t, ++kv_n) {
-          const int stage = kv_n & 1;
-          const uint32_t ph = ((kv_n >> 1) & 1) ^ 1;
-          ok = warp_wait(&bar.k_empty[stage], ph, err, kTimeout);
-          if (!ok) break;
-          put(k_s + stage * C::kOperand);
-          fence_proxy_async_smem();
-          mbar_arrive(&bar.k_full[stage]);
-          fetch(p.pg.v, t, lim_max);
-          ok = warp_wait(&bar.v_empty[stage], ph, err, kTimeout);
-          if (!ok) break;
-          if (t == t0 && !reset_marks(seg)) {
-            ok = false;
-            break;
-          }
-          if (lim_min < lim_max && (t + 1) * TILE > lim_min) {
+    };
+    uint32_t n = 0;
+    if (w.more()) {
+      const int lim = limit();
+      get_pages(w.t0, lim, true);
+      fetch(w.t0, lim);
+    }
+    while (ok && w.more()) {
+      const int lim_min = row_limit(p, w.it.q, w.it.row_lo), lim_max = limit();
+      const int seg = w.seg, t0 = w.t0, t1 = w.t1;
+      for (int t = t0; t < t1; ++t, ++n) {
+        const int stage = n & 1;
+        uint8_t* const dst = ring + stage * C::kOperand;
+        ok = warp_wait(&empty[stage], ((n >> 1) & 1) ^ 1, err, kTimeout);
+        if (ok && is_v && t == t0) ok = reset_marks(seg);
+        if (!ok) break;
+        const bool edge = is_v && lim_min < lim_max && (t + 1) * TILE > lim_min;
+        if constexpr (KV == KV_E4M3) {
+          if (edge) {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
               const int pos = t * TILE + r0 + i * RPI;
@@ -978,73 +915,40 @@ __global__ void __launch_bounds__(512, 1) kv_tile_kernel(const __grid_constant__
               x[i] = make_uint4(v[0], v[1], v[2], v[3]);
             }
           }
-          put(v_s + stage * C::kOperand);
-          fence_proxy_async_smem();
-          mbar_arrive(&bar.v_full[stage]);
-          // the keys of the next tile of this item, or of the next item's first
-          const bool same = t + 1 < t1;
-          if (!same) w.next();
-          if (same || w.more()) {
-            const int nt = same ? t + 1 : w.t0;
-            const int lim = same ? lim_max : row_limit(p, w.it.q, w.it.row_lo + w.it.rows - 1);
-            get_pages(w.it, w.head, nt, lim, !same);
-            fetch(p.pg.k, nt, lim);
-          }
-        }
-      }
-    } else {
-      // 16-bit pages need no conversion: asynchronous copies, the next tile's keys ahead of this one's arrival
-      auto issue = [&](const void* base, uint8_t* dst, int tile, int lim) {
+          const int first = (c / 4) & 1;  // lanes of the two planes take turns: no bank twice
+          uint8_t* const row0 = dst + (c / 4) * C::kPlane + r0 * 128;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const int r = r0 + i * RPI;
-          const bool in = tile * TILE + r < lim;
-          const uint8_t* src = static_cast<const uint8_t*>(base) + (in ? source(i) : 0);
-          const uint32_t to = smem_u32(dst) + (c / 8) * C::kPlane + r * 128 + 16 * ((c % 8) ^ (r & 7));
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(src), "r"(in ? 16 : 0) : "memory");
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-      };
-      if (w.more()) {
-        const int lim = row_limit(p, w.it.q, w.it.row_lo + w.it.rows - 1);
-        get_pages(w.it, w.head, w.t0, lim, true);
-        issue(p.pg.k, k_s, w.t0, lim);  // the ring is empty
-        issue(p.pg.v, v_s, w.t0, lim);
-      }
-      while (ok && w.more()) {
-        const int lim_min = row_limit(p, w.it.q, w.it.row_lo);
-        const int lim_max = row_limit(p, w.it.q, w.it.row_lo + w.it.rows - 1);
-        const int seg = w.seg;
-        const int t0 = w.t0, t1 = w.t1;
-        for (int t = t0; t < t1; ++t, ++kv_n) {
-          const int stage = kv_n & 1, next = (kv_n + 1) & 1;
-          const uint32_t ph = (((kv_n + 1) >> 1) & 1) ^ 1;
-          const bool same = t + 1 < t1;
-          if (!same) w.next();  // this tile's item is left: only its limits are used below
-          const bool more = same || w.more();
-          const int nt = same ? t + 1 : w.t0;
-          const int nl = same ? lim_max : more ? row_limit(p, w.it.q, w.it.row_lo + w.it.rows - 1) : 0;
-          if (more) {
-            get_pages(w.it, w.head, nt, nl, !same);
-            ok = warp_wait(&bar.k_empty[next], ph, err, kTimeout);
-            if (!ok) break;
-            issue(p.pg.k, k_s + next * C::kOperand, nt, nl);
-            asm volatile("cp.async.wait_group 1;" ::: "memory");
-          } else {
-            asm volatile("cp.async.wait_group 0;" ::: "memory");
+          for (int i = 0; i < N; ++i) {
+            const uint32_t v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+            uint32_t h[8];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) h[2 * e] = e4m3_pair<0>(v[e]), h[2 * e + 1] = e4m3_pair<1>(v[e]);
+            const uint4 a = make_uint4(h[0], h[1], h[2], h[3]), b = make_uint4(h[4], h[5], h[6], h[7]);
+            uint8_t* const row = row0 + i * RPI * 128;
+            static_assert(RPI % 8 == 0, "the swizzle of a thread's rows is one");
+            const int ca = (2 * (c % 4)) ^ (r0 & 7), cb = (2 * (c % 4) + 1) ^ (r0 & 7);
+            *reinterpret_cast<uint4*>(row + 16 * (first ? cb : ca)) = first ? b : a;
+            *reinterpret_cast<uint4*>(row + 16 * (first ? ca : cb)) = first ? a : b;
           }
-          if (t == t0 && !reset_marks(seg)) {
-            ok = false;
-            break;
+        } else {
+          // 16-bit pages need no conversion
+          uint8_t* const mine = dst + (c / 8) * C::kPlane + r0 * 128 + 16 * ((c % 8) ^ (r0 & 7));
+          static_assert(RPI % 8 == 0, "the swizzle of a thread's rows is one");
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            const bool in = t * TILE + r0 + i * RPI < lim_max;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(mine + i * RPI * 128)),
+                         "l"(in ? source(i) : base), "r"(in ? 16 : 0)
+                         : "memory");
           }
-          if (lim_min < lim_max && (t + 1) * TILE > lim_min) {
+          asm volatile("cp.async.wait_all;" ::: "memory");
+          if (edge) {
 #pragma unroll 1
             for (int i = 0; i < N; ++i) {
-              const int r = r0 + i * RPI, pos = t * TILE + r;
-              uint4* at = reinterpret_cast<uint4*>(v_s + stage * C::kOperand + (c / 8) * C::kPlane + r * 128 + 16 * ((c % 8) ^ (r & 7)));
-              const uint4 x = *at;  // this thread's own copy
-              uint32_t v[4] = {x.x, x.y, x.z, x.w};
-              bool found_bad = false;
+              const int pos = t * TILE + r0 + i * RPI;
+              uint4* const at = reinterpret_cast<uint4*>(mine + i * RPI * 128);  // this thread's own copy
+              uint32_t v[4] = {at->x, at->y, at->z, at->w};
+              bool any = false;
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 constexpr uint32_t kExp = kBf ? 0x7f807f80u : 0x7c007c00u;
@@ -1053,25 +957,25 @@ __global__ void __launch_bounds__(512, 1) kv_tile_kernel(const __grid_constant__
                   for (int b = 0; b < 2; ++b)
                     if ((bad >> (16 * b)) & 1u) mark(seg, pos, 8 * c + 2 * e + b);
                   v[e] &= ~bad;
-                  found_bad = true;
+                  any = true;
                 }
               }
-              if (found_bad) *at = make_uint4(v[0], v[1], v[2], v[3]);
+              if (any) *at = make_uint4(v[0], v[1], v[2], v[3]);
             }
           }
-          fence_proxy_async_smem();
-          mbar_arrive(&bar.k_full[stage]);
-          mbar_arrive(&bar.v_full[stage]);
-          if (more) {
-            ok = warp_wait(&bar.v_empty[next], ph, err, kTimeout);
-            if (!ok) break;
-            issue(p.pg.v, v_s + next * C::kOperand, nt, nl);
-          }
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(&full[stage]);
+        // the next tile of this item, or the next item's first
+        const bool same = t + 1 < t1;
+        if (!same) w.next();
+        if (same || w.more()) {
+          const int next = same ? t + 1 : w.t0, lim = same ? lim_max : limit();
+          get_pages(next, lim, !same);
+          fetch(next, lim);
         }
       }
-      asm volatile("cp.async.wait_all;" ::: "memory");
     }
-  }
   } else {
     // ---- softmax of one half
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kSoftmaxRegs));
@@ -1082,19 +986,79 @@ __global__ void __launch_bounds__(512, 1) kv_tile_kernel(const __grid_constant__
     uint32_t ph_s = 0, ph_o = 0;
     bool ok = true;
     int4 begun = make_int4(0, 0, 0, 0);
-    for (; ok && w.more(); w.next()) {
-      const Item& it = w.it;
-      const bool whole = w.whole();
+    // the warp's 32 rows of queries: HD / 8 lanes a row, all in flight at once
+    constexpr int LPQ = HD / 8, RPL = 32 / LPQ, NQ = 32 / RPL;
+    const int sub = lane % LPQ;
+    uint4 qx[NQ];
+    auto fetch_queries = [&]() {
+      const int rows = w.more() ? w.it.rows : 0;
+      const int tok0 = w.it.row_lo / p.group, g0 = w.it.row_lo - tok0 * p.group;
+      const uint16_t* const q0 = p.q + (int64_t)(w.it.q.row0 + tok0) * p.q_stride + (int64_t)w.head * p.group * HD + 8 * sub;
+#pragma unroll
+      for (int i = 0; i < NQ; ++i) {
+        const int r = half * 128 + quarter * 32 + i * RPL + lane / LPQ;
+        qx[i] = make_uint4(0, 0, 0, 0);
+        if (r < rows) {
+          const int tok = (int)(((uint32_t)(g0 + r) * (uint64_t)p.group_magic) >> 28);  // (g0 + r) / group
+          const uint16_t* s = q0 + tok * p.q_stride + (g0 + r - tok * p.group) * HD;
+          if (p.vec_q16)
+            qx[i] = __ldg(reinterpret_cast<const uint4*>(s));
+          else
+            qx[i] = make_uint4(s[0] | (uint32_t)s[1] << 16, s[2] | (uint32_t)s[3] << 16, s[4] | (uint32_t)s[5] << 16,
+                               s[6] | (uint32_t)s[7] << 16);
+        }
+      }
+    };
+    fetch_queries();
+    while (ok && w.more()) {
+      const int seg = w.seg, rows = w.it.rows;
+      const bool active = half * 128 < rows, live = my < rows, whole = w.whole();
       if (!whole && w.t0 == 0) begun = w.begun();
-      if (half * 128 >= it.rows) {
-        mbar_arrive(&bar.read[w.seg & 3]);
+      if (!active) {
+        mbar_arrive(&bar.q_full);
+        mbar_arrive(&bar.read[seg & 3]);
+        w.next();
+        fetch_queries();
         continue;
       }
-      const bool live = my < it.rows;
-      const int row = it.row_lo + my;
-      const int lim_all = row_limit(p, it.q, it.row_lo + it.rows - 1);
-      const int lim = live ? row_limit(p, it.q, row) : lim_all;
-      const int lim_warp = row_limit(p, it.q, it.row_lo + min(it.rows - 1, half * 128 + quarter * 32));
+      // queries into the operand; rows are scaled into [-1, 1] by a power of two for f16 products
+      float factor = p.scale_log2;
+      {
+        uint8_t* const dst = q_s + half * C::kOperand + (sub / 8) * C::kPlane + (quarter * 32 + lane / LPQ) * 128;
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) {
+          uint32_t v[4] = {qx[i].x, qx[i].y, qx[i].z, qx[i].w};
+          if (!(kBf && p.is_bf16)) {
+            float inv = 1.f;
+            if (!kBf) {
+              // magnitudes compare as integers
+              uint32_t a = __vmaxu2(__vmaxu2(v[0] & 0x7fff7fffu, v[1] & 0x7fff7fffu), __vmaxu2(v[2] & 0x7fff7fffu, v[3] & 0x7fff7fffu));
+#pragma unroll
+              for (int o = LPQ / 2; o; o >>= 1) a = __vmaxu2(a, __shfl_xor_sync(0xffffffffu, a, o));
+              a = max(a & 0xffffu, a >> 16);
+              const float amax = p.is_bf16 ? __uint_as_float(a << 16) : __half2float(__ushort_as_half((uint16_t)a));
+              const int e = min(max((int)(__float_as_uint(amax) >> 23) - 126, -100), 100);
+              inv = pow2i(-e);
+              const int theirs = __shfl_sync(0xffffffffu, e, (lane % RPL) * LPQ);
+              if (lane / RPL == i) factor = p.scale_log2 * pow2i(theirs);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float2 f = p.is_bf16 ? make_float2(__uint_as_float(v[k] << 16), __uint_as_float(v[k] & 0xffff0000u))
+                                         : __half22float2(*reinterpret_cast<const __half2*>(&v[k]));
+              v[k] = pack2<kBf>(f.x * inv, f.y * inv);
+            }
+          }
+          const int r = quarter * 32 + i * RPL + lane / LPQ;
+          *reinterpret_cast<uint4*>(dst + i * RPL * 128 + 16 * ((sub % 8) ^ (r & 7))) = make_uint4(v[0], v[1], v[2], v[3]);
+        }
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(&bar.q_full);
+      const int row = w.it.row_lo + my;
+      const int lim_all = row_limit(p, w.it.q, w.it.row_lo + rows - 1);
+      const int lim = live ? row_limit(p, w.it.q, row) : lim_all;
+      const int lim_warp = row_limit(p, w.it.q, w.it.row_lo + min(rows - 1, half * 128 + quarter * 32));
       float m = -INFINITY, l = 0.f;  // reference of the weights, sum
       // scale exponents of a tile's four 32-position blocks: lanes 0-3, a tile ahead
       auto get_scales = [&](int tile) {
@@ -1102,7 +1066,7 @@ __global__ void __launch_bounds__(512, 1) kv_tile_kernel(const __grid_constant__
         const uint32_t b = tile * (TILE / 32) + (lane & 3);
         if (KV == KV_E4M3 && (int)b * 32 < lim_all) {
           const uint32_t slot = kv_slot(p.pg, b);
-          int64_t page = p.b.table[it.seq * p.b.max_pages + slot];
+          int64_t page = p.b.table[w.it.seq * p.b.max_pages + slot];
           if (page < 0 || page >= p.pg.n_pages) page = 0;
           const int64_t at = (page * p.pg.n_head_kv + w.head) * p.pg.page_blocks + (b - slot * p.pg.page_blocks);
           e = p.pg.k_scale[at] | p.pg.v_scale[at] << 8;
@@ -1110,12 +1074,10 @@ __global__ void __launch_bounds__(512, 1) kv_tile_kernel(const __grid_constant__
         return e;
       };
       int sc_next = get_scales(w.t0);
-      ok = warp_wait(&bar.q_full, w.seg & 1, err, kTimeout);
-      if (!ok) break;
-      const float factor = factor_s[w.seg & 1][my];
-      for (int t = w.t0; t < w.t1; ++t) {
+      const int t0 = w.t0, t1 = w.t1;
+      for (int t = t0; t < t1; ++t) {
         const int sc = sc_next;
-        if (t + 1 < w.t1) sc_next = get_scales(t + 1);
+        if (t + 1 < t1) sc_next = get_scales(t + 1);
         float c[4], ev[4];
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
@@ -1142,12 +1104,14 @@ __global__ void __launch_bounds__(512, 1) kv_tile_kernel(const __grid_constant__
         float mx = -INFINITY;
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-          float top[4];
+          float top[2] = {__uint_as_float(x[b][0]), __uint_as_float(x[b][1])};
 #pragma unroll
-          for (int i = 0; i < 4; ++i) top[i] = __uint_as_float(x[b][i]);
-#pragma unroll
-          for (int i = 4; i < 32; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(x[b][i]));
-          mx = fmaxf(mx, fmaf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), c[b], ev[b]));
+          for (int i = 2; i < 30; i += 4) {
+            top[0] = max3(top[0], __uint_as_float(x[b][i]), __uint_as_float(x[b][i + 1]));
+            top[1] = max3(top[1], __uint_as_float(x[b][i + 2]), __uint_as_float(x[b][i + 3]));
+          }
+          top[0] = max3(top[0], __uint_as_float(x[b][30]), __uint_as_float(x[b][31]));
+          mx = fmaxf(mx, fmaf(fmaxf(top[0], top[1]), c[b], ev[b]));
         }
         float shrink = 1.f;
         if (mx > m + 8.f || m == -INFINITY) {
@@ -1156,7 +1120,7 @@ __global__ void __launch_bounds__(512, 1) kv_tile_kernel(const __grid_constant__
           m = to;
           l *= shrink;
         }
-        if (t > w.t0 && __any_sync(0xffffffffu, shrink != 1.f)) {
+        if (t > t0 && __any_sync(0xffffffffu, shrink != 1.f)) {
           // the products of the tile before have ended: the scores' arrival counts them
 #pragma unroll 1
           for (int d = 0; d < HD; d += 16) {
@@ -1171,50 +1135,53 @@ __global__ void __launch_bounds__(512, 1) kv_tile_kernel(const __grid_constant__
         const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-          const float off = ev[b] - base;
-          float sum[2] = {0.f, 0.f};
+          const uint64_t c2 = pair(c[b], c[b]), off2 = pair(ev[b] - base, ev[b] - base);
+          uint64_t sum = pair(0.f, 0.f);
           uint32_t pk[16];
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
-            const float a = ex2(fmaf(__uint_as_float(x[b][i]), c[b], off)), d = ex2(fmaf(__uint_as_float(x[b][i + 1]), c[b], off));
-            sum[0] += a, sum[1] += d;
+            float a, d;
+            unpair(fma2(pair(__uint_as_float(x[b][i]), __uint_as_float(x[b][i + 1])), c2, off2), a, d);
+            a = ex2(a), d = ex2(d);
+            sum = add2(sum, pair(a, d));
             pk[i / 2] = pack2<kBf>(a, d);
           }
           tmem_st16(s_addr + 16 * b, pk);
-          l = fmaf(sum[0] + sum[1], KV == KV_E4M3 ? pow2i(-(int)ev[b]) : 1.f, l);
+          float a, d;
+          unpair(sum, a, d);
+          l = fmaf(a + d, KV == KV_E4M3 ? pow2i(-(int)ev[b]) : 1.f, l);
         }
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(&bar.p_full[half]);
       }
       if (!ok) break;
+      const int head = w.head, group_row = row % p.group;
+      const int64_t token = w.it.q.row0 + row / p.group;
+      w.next();
+      fetch_queries();  // on their way during the last product and the output
       ok = warp_wait(&bar.o_full[half], ph_o, err, kTimeout);
       if (!ok) break;
       ph_o ^= 1;
       tc_fence_after();
-      const bool marked = *const_cast<volatile int*>(&any_not_finite[w.seg & 3]) != 0;
-      float* part = p.part + (int64_t)(2 * blockIdx.x + (w.t0 == 0 ? 1 : 0)) * C::kPart;
+      const bool marked = *const_cast<volatile int*>(&any_not_finite[seg & 3]) != 0;
+      float* const part = p.part + (int64_t)(2 * blockIdx.x + (t0 == 0 ? 1 : 0)) * C::kPart;
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      const int64_t at = (int64_t)(it.q.row0 + row / p.group) * p.out_stride + (int64_t)(w.head * p.group + row % p.group) * HD;
-#pragma unroll
-      for (int d0 = 0; d0 < HD; d0 += 64) {
-        uint32_t x[64];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) tmem_ld32(o_addr + d0 + 32 * i, reinterpret_cast<uint32_t(&)[32]>(x[32 * i]));
+      uint16_t* const out = p.out + token * p.out_stride + (int64_t)(head * p.group + group_row) * HD;
+#pragma unroll 1
+      for (int d0 = 0; d0 < HD; d0 += 32) {
+        uint32_t x[32];
+        tmem_ld32(o_addr + d0, x);
         tmem_wait_ld();
         if (marked) {
-#pragma unroll 1
-          for (int i = 0; i < 64; ++i)
-            if (*const_cast<volatile int*>(&not_finite_from[w.seg & 3][d0 + i]) < lim) {
 #pragma unroll
-              for (int e = 0; e < 64; ++e)
-                if (e == i) x[e] = 0x7fc00000u;
-            }
+          for (int i = 0; i < 32; ++i)
+            if (*const_cast<volatile int*>(&not_finite_from[seg & 3][d0 + i]) < lim) x[i] = 0x7fc00000u;
         }
         if (!live) continue;
         if (whole) {
 #pragma unroll
-          for (int i = 0; i < 64; i += 8) {
+          for (int i = 0; i < 32; i += 8) {
             uint32_t h[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -1222,35 +1189,35 @@ __global__ void __launch_bounds__(512, 1) kv_tile_kernel(const __grid_constant__
               h[e] = p.is_bf16 ? pack2<true>(a, b) : pack2<false>(a, b);
             }
             if (p.vec_out16) {
-              *reinterpret_cast<uint4*>(p.out + at + d0 + i) = make_uint4(h[0], h[1], h[2], h[3]);
+              *reinterpret_cast<uint4*>(out + d0 + i) = make_uint4(h[0], h[1], h[2], h[3]);
             } else {
 #pragma unroll
-              for (int e = 0; e < 8; ++e) p.out[at + d0 + i + e] = (uint16_t)(h[e / 2] >> (16 * (e & 1)));
+              for (int e = 0; e < 8; ++e) out[d0 + i + e] = (uint16_t)(h[e / 2] >> (16 * (e & 1)));
             }
           }
         } else {
           float4* to = reinterpret_cast<float4*>(part + my * HD + d0);
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
+          for (int i = 0; i < 8; ++i)
             to[i] = make_float4(__uint_as_float(x[4 * i]), __uint_as_float(x[4 * i + 1]), __uint_as_float(x[4 * i + 2]),
                                 __uint_as_float(x[4 * i + 3]));
         }
       }
       if (live) {
-        if (whole)
-          store_lse(p, it.q, row, w.head, m, l);
-        else
+        if (!whole)
           part[R * HD + 2 * my] = m, part[R * HD + 2 * my + 1] = l;
+        else if (p.lse)
+          p.lse[token * p.n_head + head * p.group + group_row] = l == 0.f ? -INFINITY : kLn2 * (m + log2f(l));
       }
       tc_fence_before();
-      mbar_arrive(&bar.read[w.seg & 3]);
+      mbar_arrive(&bar.read[seg & 3]);
     }
     if (tid == 0) p.desc[blockIdx.x] = begun;
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 12) tmem_dealloc(tmem, 512);
+  if (warp == 16) tmem_dealloc(tmem, 512);
   pdl_trigger();
 }
 
@@ -1412,6 +1379,7 @@ extern "C" dmoe_status dmoe_kv_attention(const dmoe_kv_cache* cache, const dmoe_
   p.is_bf16 = a->type == DMOE_TYPE_BF16;
   p.n_head = a->n_head;
   p.group = group;
+  p.group_magic = (uint32_t)(((1u << 28) + group - 1) / group);
   p.block_length = a->block_length;
   p.vec_q = ((reinterpret_cast<uintptr_t>(a->q) | (uintptr_t)(2 * a->q_stride)) & 7u) == 0;
   p.vec_q16 = ((reinterpret_cast<uintptr_t>(a->q) | (uintptr_t)(2 * a->q_stride)) & 15u) == 0;
