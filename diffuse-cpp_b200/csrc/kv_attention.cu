@@ -30,7 +30,15 @@ namespace dmoe {
 
 namespace {
 
+constexpr int kMaxGrid = 148;  // one CTA an SM
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+// An item that a CTA begins and does not end
+struct Spanning {
+  int last;  // CTA that ends it; -1: there is none
+  int row0, row_lo, rows, head;  // the sequence's first row, the item's rows [row_lo, row_lo + rows) of q_len * group
+  int pad[3];
+};
 
 struct AttnParams {
   KvPages pg;
@@ -48,7 +56,7 @@ struct AttnParams {
   float scale_log2;  // scale * log2(e)
   uint32_t* wait_err;  // word that bounded waits report to
   float* part;       // partial triples, slot = 2 * CTA + (the item begins in this CTA)
-  int4* desc;        // [CTA] {item, head, last CTA, 1} of the item this CTA begins and does not end
+  struct Spanning* desc;  // [CTA]
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -102,9 +110,9 @@ __device__ __forceinline__ int row_limit(const AttnParams& p, const KvSeq& q, in
 template <int R, int TILE>
 __device__ __forceinline__ Item item_of(const AttnParams& p, int u) {
   Item it;
-  it.seq = u / p.n_qt;
+  it.seq = p.n_qt == 1 ? u : u / p.n_qt;
   it.q = kv_sequence(p.b, p.pg, it.seq);
-  it.row_lo = (u % p.n_qt) * R;
+  it.row_lo = (u - it.seq * p.n_qt) * R;
   it.rows = min(R, it.q.q_len * p.group - it.row_lo);
   it.tiles = 0;
   if (it.rows > 0) it.tiles = max(1, (row_limit(p, it.q, it.row_lo + it.rows - 1) + TILE - 1) / TILE);
@@ -114,7 +122,8 @@ __device__ __forceinline__ Item item_of(const AttnParams& p, int u) {
 // Beginning and ending an item costs about as much as OV tiles. An item of t tiles is OV + t units long, and
 // the units of all items are numbered through; its tiles are the last t.
 struct Run {       // a CTA's run of units
-  int u, head;     // first item
+  Item it;         // first item
+  int u, head;
   int unit;        // first unit within it
   int left;        // units of the run (2^31 tiles would take an hour: no workload has them)
   int chunk;       // units of every run but the last
@@ -154,9 +163,10 @@ __device__ __forceinline__ Run find_run(const AttnParams& p, int64_t* sums, Run*
   before *= heads;
   if (first < total && first >= before && first < before + mine * heads) {
     for (int64_t u = u0; u < u1; ++u) {
-      const int t = item_of<R, TILE>(p, (int)u).tiles;
-      const int64_t w = t ? t + OV : 0;
+      const Item it = item_of<R, TILE>(p, (int)u);
+      const int64_t w = it.tiles ? it.tiles + OV : 0;
       if (first < before + w * heads) {
+        found->it = it;
         found->u = (int)u;
         found->head = (int)((first - before) / w);
         found->unit = (int)((first - before) % w);
@@ -178,20 +188,19 @@ __device__ __forceinline__ Run find_run(const AttnParams& p, int64_t* sums, Run*
 template <int R, int TILE, int OV>
 struct Walk {
   const AttnParams& p;
-  Item it{};
+  Item it;
   int u, head, seg = -1, t0 = 0, t1 = 0;
   int unit, left, chunk;
   int64_t at;
   __device__ __forceinline__ Walk(const AttnParams& p_, const Run& r)
-      : p(p_), u(r.u), head(r.head), unit(r.unit), left(r.left), chunk(r.chunk), at(r.first) {
-    if (left > 0) it = item_of<R, TILE>(p, u);
+      : p(p_), it(r.it), u(r.u), head(r.head), unit(r.unit), left(r.left), chunk(r.chunk), at(r.first) {
     settle();
   }
   __device__ __forceinline__ bool more() const { return left > 0; }
   __device__ __forceinline__ bool whole() const { return t0 == 0 && t1 == it.tiles; }
-  // {item, head, last CTA that has a part of it, 1}: for an item that this CTA begins and does not end
-  __device__ __forceinline__ int4 begun() const {
-    return make_int4(u, head, (int)((at - unit + OV + it.tiles - 1) / chunk), 1);
+  // for an item that this CTA begins and does not end
+  __device__ __forceinline__ Spanning begun() const {
+    return {(int)((at - unit + OV + it.tiles - 1) / chunk), it.q.row0, it.row_lo, it.rows, head, {0, 0, 0}};
   }
   __device__ __forceinline__ void next() {
     advance();
@@ -303,17 +312,17 @@ __device__ __forceinline__ void load_q4(const AttnParams& p, int64_t at, float (
   }
 }
 
-__device__ __forceinline__ void store_out(const AttnParams& p, const KvSeq& q, int row, int head, int d, int hd, float x) {
-  const int64_t at = (int64_t)(q.row0 + row / p.group) * p.out_stride + (int64_t)(head * p.group + row % p.group) * hd + d;
+__device__ __forceinline__ void store_out(const AttnParams& p, int row0, int row, int head, int d, int hd, float x) {
+  const int64_t at = (int64_t)(row0 + row / p.group) * p.out_stride + (int64_t)(head * p.group + row % p.group) * hd + d;
   if (p.is_bf16)
     p.out[at] = __bfloat16_as_ushort(__float2bfloat16_rn(x));
   else
     p.out[at] = __half_as_ushort(__float2half_rn(x));
 }
 
-__device__ __forceinline__ void store_lse(const AttnParams& p, const KvSeq& q, int row, int head, float m, float l) {
+__device__ __forceinline__ void store_lse(const AttnParams& p, int row0, int row, int head, float m, float l) {
   if (p.lse)
-    p.lse[(int64_t)(q.row0 + row / p.group) * p.n_head + head * p.group + row % p.group] =
+    p.lse[(int64_t)(row0 + row / p.group) * p.n_head + head * p.group + row % p.group] =
         l == 0.f ? -INFINITY : kLn2 * (m + log2f(l));
 }
 
@@ -355,7 +364,7 @@ __global__ void __launch_bounds__(256, 1) kv_rows_kernel(const __grid_constant__
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
 
   pdl_wait();
-  int4 begun = make_int4(0, 0, 0, 0);
+  Spanning begun = {-1, 0, 0, 0, 0, {0, 0, 0}};
   for (Walk<R, TILE, C::OV> w(p, find_run<R, TILE, C::OV, 256>(p, sums, &found)); w.more(); w.next()) {
     const Item& it = w.it;
     const int head = w.head;
@@ -646,8 +655,8 @@ __global__ void __launch_bounds__(256, 1) kv_rows_kernel(const __grid_constant__
         ll = fmaf(ml[(k * R + r) * 2 + 1], f, ll);
       }
       if (whole) {
-        store_out(p, it.q, it.row_lo + r, head, d, HD, ll == 0.f ? 0.f : acc / ll);
-        if (d == 0) store_lse(p, it.q, it.row_lo + r, head, mm, ll);
+        store_out(p, it.q.row0, it.row_lo + r, head, d, HD, ll == 0.f ? 0.f : acc / ll);
+        if (d == 0) store_lse(p, it.q.row0, it.row_lo + r, head, mm, ll);
       } else {
         part[r * HD + d] = acc;
         if (d == 0) part[R * HD + 2 * r] = mm, part[R * HD + 2 * r + 1] = ll;
@@ -684,7 +693,8 @@ struct TileCfg {
   static constexpr int kPlane = 128 * 128;             // 64 elements of 128 rows
   static constexpr int kOperand = HD / 64 * kPlane;    // bytes of a 128-row operand
   static constexpr int kStages = 2;
-  static constexpr size_t kSmem = 1024 + (2 + 2 * kStages) * (size_t)kOperand;
+  static constexpr int kOutWarp = 32 * 64;             // staging of 32 columns of a warp's 32 output rows
+  static constexpr size_t kSmem = 1024 + (2 + 2 * kStages) * (size_t)kOperand + 8 * kOutWarp;
   static constexpr int kPart = R * (HD + 2);
 };
 
@@ -711,10 +721,14 @@ __global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__
   __shared__ Run found;
   __shared__ int not_finite_from[4][HD];  // [item of the run & 3][d]: first position whose value is not finite
   __shared__ int any_not_finite[4];
+  // scale exponents [value][tile of the run & 3][32-position block]. Written before the tile's arrival; the
+  // slot is free again when the tile two on has been multiplied by both halves' queries
+  __shared__ int scale_s[2][4][4];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* q_s = smem;                                 // [half] operands
   uint8_t* k_s = q_s + 2 * C::kOperand;                // [stage]
   uint8_t* v_s = k_s + C::kStages * C::kOperand;       // [stage]
+  uint8_t* out_s = v_s + C::kStages * C::kOperand;     // [softmax warp]
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
   if (warp == 16) {
@@ -872,8 +886,14 @@ __global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__
     };
     auto limit = [&]() { return row_limit(p, w.it.q, w.it.row_lo + w.it.rows - 1); };
     uint4 x[KV == KV_E4M3 ? N : 1];  // 8-bit pages: the next tile, on its way
+    int scale = 0;                   // and the exponent of its block `lane` (threads 0-3)
     auto fetch = [&](int tile, int lim) {
       if constexpr (KV == KV_E4M3) {
+        scale = 0;
+        if (lt < 4 && tile * TILE + 32 * lt < lim) {
+          const int64_t row = lt == 0 ? first_row[0] : lt == 1 ? first_row[1] : lt == 2 ? first_row[2] : first_row[3];
+          scale = (int)(is_v ? p.pg.v_scale : p.pg.k_scale)[row / kScaleBlock] - 127;
+        }
 #pragma unroll
         for (int i = 0; i < N; ++i) {
           x[i] = make_uint4(0, 0, 0, 0);
@@ -898,6 +918,7 @@ __global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__
         if (!ok) break;
         const bool edge = is_v && lim_min < lim_max && (t + 1) * TILE > lim_min;
         if constexpr (KV == KV_E4M3) {
+          if (lt < 4) *const_cast<volatile int*>(&scale_s[is_v][n & 3][lt]) = scale;
           if (edge) {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
@@ -985,31 +1006,34 @@ __global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__
     const uint32_t s_addr = tmem_addr(tmem, quarter * 32, half * 128), o_addr = tmem_addr(tmem, quarter * 32, 256 + half * 128);
     uint32_t ph_s = 0, ph_o = 0;
     bool ok = true;
-    int4 begun = make_int4(0, 0, 0, 0);
-    // the warp's 32 rows of queries: HD / 8 lanes a row, all in flight at once
-    constexpr int LPQ = HD / 8, RPL = 32 / LPQ, NQ = 32 / RPL;
-    const int sub = lane % LPQ;
-    uint4 qx[NQ];
+    Spanning begun = {-1, 0, 0, 0, 0, {0, 0, 0}};
+    // the warp's 32 rows of queries, HD / 8 lanes a row, copied into the operand as they are
+    constexpr int LPQ = HD / 8, RPL = 32 / LPQ;
+    uint8_t* const q_warp = q_s + half * C::kOperand + quarter * 32 * 128;
     auto fetch_queries = [&]() {
-      const int rows = w.more() ? w.it.rows : 0;
-      const int tok0 = w.it.row_lo / p.group, g0 = w.it.row_lo - tok0 * p.group;
+      if (!w.more() || half * 128 >= w.it.rows) return;
+      const int tok0 = w.it.row_lo / p.group, g0 = w.it.row_lo - tok0 * p.group, sub = lane % LPQ;
       const uint16_t* const q0 = p.q + (int64_t)(w.it.q.row0 + tok0) * p.q_stride + (int64_t)w.head * p.group * HD + 8 * sub;
+#pragma unroll 2
+      for (int r = lane / LPQ; r < 32; r += RPL) {
+        const int row = g0 + half * 128 + quarter * 32 + r;
+        const int tok = (int)((row * (uint64_t)p.group_magic) >> 28);  // row / group
+        const bool in = half * 128 + quarter * 32 + r < w.it.rows;
+        const uint16_t* const src = in ? q0 + tok * p.q_stride + (row - tok * p.group) * HD : p.q;
+        uint8_t* const dst = q_warp + (sub / 8) * C::kPlane + r * 128 + 16 * ((sub % 8) ^ (r & 7));
+        if (p.vec_q16) {
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(in ? 16 : 0) : "memory");
+        } else {
+          uint16_t h[8];
 #pragma unroll
-      for (int i = 0; i < NQ; ++i) {
-        const int r = half * 128 + quarter * 32 + i * RPL + lane / LPQ;
-        qx[i] = make_uint4(0, 0, 0, 0);
-        if (r < rows) {
-          const int tok = (int)(((uint32_t)(g0 + r) * (uint64_t)p.group_magic) >> 28);  // (g0 + r) / group
-          const uint16_t* s = q0 + tok * p.q_stride + (g0 + r - tok * p.group) * HD;
-          if (p.vec_q16)
-            qx[i] = __ldg(reinterpret_cast<const uint4*>(s));
-          else
-            qx[i] = make_uint4(s[0] | (uint32_t)s[1] << 16, s[2] | (uint32_t)s[3] << 16, s[4] | (uint32_t)s[5] << 16,
-                               s[6] | (uint32_t)s[7] << 16);
+          for (int e = 0; e < 8; ++e) h[e] = in ? src[e] : (uint16_t)0;
+          *reinterpret_cast<uint4*>(dst) = make_uint4(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16,
+                                                      h[4] | (uint32_t)h[5] << 16, h[6] | (uint32_t)h[7] << 16);
         }
       }
     };
     fetch_queries();
+    uint32_t n = 0;  // tiles
     while (ok && w.more()) {
       const int seg = w.seg, rows = w.it.rows;
       const bool active = half * 128 < rows, live = my < rows, whole = w.whole();
@@ -1017,40 +1041,43 @@ __global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__
       if (!active) {
         mbar_arrive(&bar.q_full);
         mbar_arrive(&bar.read[seg & 3]);
+        n += w.t1 - w.t0;
         w.next();
         fetch_queries();
         continue;
       }
-      // queries into the operand; rows are scaled into [-1, 1] by a power of two for f16 products
+      // a thread turns its row into the products' type; f16 products: scaled into [-1, 1] by a power of two
       float factor = p.scale_log2;
-      {
-        uint8_t* const dst = q_s + half * C::kOperand + (sub / 8) * C::kPlane + (quarter * 32 + lane / LPQ) * 128;
-#pragma unroll
-        for (int i = 0; i < NQ; ++i) {
-          uint32_t v[4] = {qx[i].x, qx[i].y, qx[i].z, qx[i].w};
-          if (!(kBf && p.is_bf16)) {
-            float inv = 1.f;
-            if (!kBf) {
-              // magnitudes compare as integers
-              uint32_t a = __vmaxu2(__vmaxu2(v[0] & 0x7fff7fffu, v[1] & 0x7fff7fffu), __vmaxu2(v[2] & 0x7fff7fffu, v[3] & 0x7fff7fffu));
-#pragma unroll
-              for (int o = LPQ / 2; o; o >>= 1) a = __vmaxu2(a, __shfl_xor_sync(0xffffffffu, a, o));
-              a = max(a & 0xffffu, a >> 16);
-              const float amax = p.is_bf16 ? __uint_as_float(a << 16) : __half2float(__ushort_as_half((uint16_t)a));
-              const int e = min(max((int)(__float_as_uint(amax) >> 23) - 126, -100), 100);
-              inv = pow2i(-e);
-              const int theirs = __shfl_sync(0xffffffffu, e, (lane % RPL) * LPQ);
-              if (lane / RPL == i) factor = p.scale_log2 * pow2i(theirs);
-            }
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const float2 f = p.is_bf16 ? make_float2(__uint_as_float(v[k] << 16), __uint_as_float(v[k] & 0xffff0000u))
-                                         : __half22float2(*reinterpret_cast<const __half2*>(&v[k]));
-              v[k] = pack2<kBf>(f.x * inv, f.y * inv);
-            }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      __syncwarp();
+      if (!(kBf && p.is_bf16)) {
+        uint8_t* const mine = q_warp + lane * 128;
+        auto piece = [&](int i) { return reinterpret_cast<uint4*>(mine + (i / 8) * C::kPlane + 16 * ((i % 8) ^ (lane & 7))); };
+        float inv = 1.f;
+        if (!kBf) {
+          uint32_t a = 0;  // magnitudes compare as integers
+#pragma unroll 4
+          for (int i = 0; i < HD / 8; ++i) {
+            const uint4 v = *piece(i);
+            a = __vmaxu2(a, __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
           }
-          const int r = quarter * 32 + i * RPL + lane / LPQ;
-          *reinterpret_cast<uint4*>(dst + i * RPL * 128 + 16 * ((sub % 8) ^ (r & 7))) = make_uint4(v[0], v[1], v[2], v[3]);
+          a = max(a & 0xffffu, a >> 16);
+          const float amax = p.is_bf16 ? __uint_as_float(a << 16) : __half2float(__ushort_as_half((uint16_t)a));
+          const int e = min(max((int)(__float_as_uint(amax) >> 23) - 126, -100), 100);
+          inv = pow2i(-e);
+          factor *= pow2i(e);
+        }
+#pragma unroll 2
+        for (int i = 0; i < HD / 8; ++i) {
+          const uint4 x = *piece(i);
+          uint32_t v[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float2 f = p.is_bf16 ? make_float2(__uint_as_float(v[k] << 16), __uint_as_float(v[k] & 0xffff0000u))
+                                       : __half22float2(*reinterpret_cast<const __half2*>(&v[k]));
+            v[k] = pack2<kBf>(f.x * inv, f.y * inv);
+          }
+          *piece(i) = make_uint4(v[0], v[1], v[2], v[3]);
         }
       }
       fence_proxy_async_smem();
@@ -1060,31 +1087,8 @@ __global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__
       const int lim = live ? row_limit(p, w.it.q, row) : lim_all;
       const int lim_warp = row_limit(p, w.it.q, w.it.row_lo + min(rows - 1, half * 128 + quarter * 32));
       float m = -INFINITY, l = 0.f;  // reference of the weights, sum
-      // scale exponents of a tile's four 32-position blocks: lanes 0-3, a tile ahead
-      auto get_scales = [&](int tile) {
-        int e = 127 | 127 << 8;
-        const uint32_t b = tile * (TILE / 32) + (lane & 3);
-        if (KV == KV_E4M3 && (int)b * 32 < lim_all) {
-          const uint32_t slot = kv_slot(p.pg, b);
-          int64_t page = p.b.table[w.it.seq * p.b.max_pages + slot];
-          if (page < 0 || page >= p.pg.n_pages) page = 0;
-          const int64_t at = (page * p.pg.n_head_kv + w.head) * p.pg.page_blocks + (b - slot * p.pg.page_blocks);
-          e = p.pg.k_scale[at] | p.pg.v_scale[at] << 8;
-        }
-        return e;
-      };
-      int sc_next = get_scales(w.t0);
       const int t0 = w.t0, t1 = w.t1;
-      for (int t = t0; t < t1; ++t) {
-        const int sc = sc_next;
-        if (t + 1 < t1) sc_next = get_scales(t + 1);
-        float c[4], ev[4];
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          const int e = __shfl_sync(0xffffffffu, sc, b);
-          c[b] = KV == KV_E4M3 ? factor * pow2i((e & 255) - 127) : factor;
-          ev[b] = KV == KV_E4M3 ? (float)((e >> 8) - 127) : 0.f;
-        }
+      for (int t = t0; t < t1; ++t, ++n) {
         ok = warp_wait(&bar.s_full[half], ph_s, err, kTimeout);
         if (!ok) break;
         ph_s ^= 1;
@@ -1092,6 +1096,12 @@ __global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__
         uint32_t x[4][32];
 #pragma unroll
         for (int b = 0; b < 4; ++b) tmem_ld32(s_addr + 32 * b, x[b]);
+        float c[4], ev[4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          c[b] = KV == KV_E4M3 ? factor * pow2i(*const_cast<volatile int*>(&scale_s[0][n & 3][b])) : factor;
+          ev[b] = KV == KV_E4M3 ? (float)*const_cast<volatile int*>(&scale_s[1][n & 3][b]) : 0.f;
+        }
         tmem_wait_ld();
         if ((t + 1) * TILE > lim_warp) {
           const int valid = lim - t * TILE;  // columns this row sees
@@ -1156,58 +1166,74 @@ __global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__
         mbar_arrive(&bar.p_full[half]);
       }
       if (!ok) break;
-      const int head = w.head, group_row = row % p.group;
-      const int64_t token = w.it.q.row0 + row / p.group;
+      const Item it = w.it;
+      const int head = w.head;
       w.next();
-      fetch_queries();  // on their way during the last product and the output
+      fetch_queries();  // the scores' last arrival: the operand is free. On their way during the last product
       ok = warp_wait(&bar.o_full[half], ph_o, err, kTimeout);
       if (!ok) break;
       ph_o ^= 1;
       tc_fence_after();
       const bool marked = *const_cast<volatile int*>(&any_not_finite[seg & 3]) != 0;
-      float* const part = p.part + (int64_t)(2 * blockIdx.x + (t0 == 0 ? 1 : 0)) * C::kPart;
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      uint16_t* const out = p.out + token * p.out_stride + (int64_t)(head * p.group + group_row) * HD;
+      // a warp's rows lie side by side in a partial, [d][row]; rows of the output go through shared memory, 32
+      // columns at a time, so that either is written in whole sectors
+      float* const part = p.part + (int64_t)(2 * blockIdx.x + (t0 == 0 ? 1 : 0)) * C::kPart + my;
+      uint8_t* const stage = out_s + warp * C::kOutWarp;
 #pragma unroll 1
       for (int d0 = 0; d0 < HD; d0 += 32) {
         uint32_t x[32];
         tmem_ld32(o_addr + d0, x);
         tmem_wait_ld();
         if (marked) {
-#pragma unroll
+#pragma unroll 1
           for (int i = 0; i < 32; ++i)
-            if (*const_cast<volatile int*>(&not_finite_from[seg & 3][d0 + i]) < lim) x[i] = 0x7fc00000u;
-        }
-        if (!live) continue;
-        if (whole) {
+            if (*const_cast<volatile int*>(&not_finite_from[seg & 3][d0 + i]) < lim) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 8) {
-            uint32_t h[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float a = l == 0.f ? 0.f : __uint_as_float(x[i + 2 * e]) * inv, b = l == 0.f ? 0.f : __uint_as_float(x[i + 2 * e + 1]) * inv;
-              h[e] = p.is_bf16 ? pack2<true>(a, b) : pack2<false>(a, b);
+              for (int e = 0; e < 32; ++e) x[e] = e == i ? 0x7fc00000u : x[e];
             }
-            if (p.vec_out16) {
-              *reinterpret_cast<uint4*>(out + d0 + i) = make_uint4(h[0], h[1], h[2], h[3]);
-            } else {
+        }
+        if (!whole) {
+          if (live) {
 #pragma unroll
-              for (int e = 0; e < 8; ++e) out[d0 + i + e] = (uint16_t)(h[e / 2] >> (16 * (e & 1)));
+            for (int i = 0; i < 32; ++i) part[(d0 + i) * R] = __uint_as_float(x[i]);
+          }
+          continue;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t h[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float a = l == 0.f ? 0.f : __uint_as_float(x[8 * i + 2 * e]) * inv, b = l == 0.f ? 0.f : __uint_as_float(x[8 * i + 2 * e + 1]) * inv;
+            h[e] = p.is_bf16 ? pack2<true>(a, b) : pack2<false>(a, b);
+          }
+          *reinterpret_cast<uint4*>(stage + lane * 64 + 16 * (i ^ ((lane >> 1) & 3))) = make_uint4(h[0], h[1], h[2], h[3]);
+        }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = 8 * i + lane / 4, of = half * 128 + quarter * 32 + r;
+          const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 64 + 16 * ((lane % 4) ^ ((r >> 1) & 3)));
+          if (of < rows) {
+            const int orow = it.row_lo + of, tok = orow / p.group;
+            uint16_t* const o = p.out + (int64_t)(it.q.row0 + tok) * p.out_stride + (int64_t)(head * p.group + orow - tok * p.group) * HD + d0 + 8 * (lane % 4);
+            if (p.vec_out16) {
+              *reinterpret_cast<uint4*>(o) = v;
+            } else {
+              const uint32_t h[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+              for (int e = 0; e < 8; ++e) o[e] = (uint16_t)(h[e / 2] >> (16 * (e & 1)));
             }
           }
-        } else {
-          float4* to = reinterpret_cast<float4*>(part + my * HD + d0);
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            to[i] = make_float4(__uint_as_float(x[4 * i]), __uint_as_float(x[4 * i + 1]), __uint_as_float(x[4 * i + 2]),
-                                __uint_as_float(x[4 * i + 3]));
         }
+        __syncwarp();
       }
       if (live) {
         if (!whole)
-          part[R * HD + 2 * my] = m, part[R * HD + 2 * my + 1] = l;
-        else if (p.lse)
-          p.lse[token * p.n_head + head * p.group + group_row] = l == 0.f ? -INFINITY : kLn2 * (m + log2f(l));
+          part[HD * R] = m, part[(HD + 1) * R] = l;
+        else
+          store_lse(p, it.q.row0, row, head, m, l);
       }
       tc_fence_before();
       mbar_arrive(&bar.read[seg & 3]);
@@ -1221,62 +1247,144 @@ __global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__
   pdl_trigger();
 }
 
-// Adds the partial triples of the item that CTA blockIdx.x of the first kernel began: those of
-// slots 2c + 1, 2(c + 1), .. 2 last. HD / 4 threads a row; GROUPS of them share the triples of one row and
-// add their sums in order (few rows: many triples each), or take a row each (GROUPS = 1).
-template <int HD, int R, int TILE, int GROUPS>
-__global__ void __launch_bounds__(8 * HD / 4) kv_combine_kernel(const __grid_constant__ AttnParams p) {
-  constexpr int kLanes = HD / 4, kRows = 8 / GROUPS;
-  __shared__ float4 acc_s[8][kLanes];
-  __shared__ float l_s[8];
+// Adds the partial triples of the items that the CTAs of the first kernel began and did not end: for CTA c's,
+// those of slots 2c + 1, 2(c + 1), .. 2 last. The pieces of all such items (PIECES each) are shared out over the
+// grid: every CTA reads all descriptors and takes every gridDim.x-th piece. Eight teams of threads take every
+// eighth triple with a running maximum each, and are joined in order.
+template <int PIECES, typename F>
+__device__ __forceinline__ void for_pieces(const AttnParams& p, int n_cta, F&& f) {
+  __shared__ Spanning begun_s[kMaxGrid];
+  __shared__ int from_s[kMaxGrid];
+  __shared__ int count_s[8];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  Spanning d{};
+  d.last = -1;
+  if (tid < n_cta) d = p.desc[tid];
+  const bool has = d.last >= 0;
+  const uint32_t mask = __ballot_sync(0xffffffffu, has);
+  if (lane == 0) count_s[warp] = __popc(mask);
+  __syncthreads();
+  int before = 0, total = 0;
+  for (int w = 0; w < 8; ++w) {
+    if (w < warp) before += count_s[w];
+    total += count_s[w];
+  }
+  if (has) {
+    const int i = before + __popc(mask & ((1u << lane) - 1));
+    begun_s[i] = d;
+    from_s[i] = tid;
+  }
+  __syncthreads();
+  for (int i = blockIdx.x; i < total * PIECES; i += gridDim.x) f(begun_s[i / PIECES], from_s[i / PIECES], i % PIECES);
+}
+
+// Few rows, triples [row][d]: a piece is a row.
+template <int HD, int R>
+__global__ void __launch_bounds__(256) kv_combine_kernel(const __grid_constant__ AttnParams p, int n_cta) {
+  constexpr int D = HD / 32;  // columns a lane
+  __shared__ float acc_s[8][HD];
+  __shared__ float m_s[8], l_s[8];
   pdl_wait();
-  const int c = blockIdx.x;
-  const int4 begun = p.desc[c];
-  if (begun.w == 0) return;
-  const Item it = item_of<R, TILE>(p, begun.x);
-  const int sub = threadIdx.x % kLanes, team = threadIdx.x / kLanes, grp = team % GROUPS;
-  const int r = blockIdx.y * kRows + team / GROUPS;
-  if (blockIdx.y * kRows >= it.rows) return;
-  const bool live = r < it.rows;
-  const int n = live ? begun.z - c + 1 : 0;
-  auto slot = [&](int k) { return p.part + (int64_t)(2 * (c + k) + (k == 0 ? 1 : 0)) * (R * (HD + 2)); };
-  float m = -INFINITY;
-  for (int k = 0; k < n; ++k) m = fmaxf(m, slot(k)[R * HD + 2 * r]);
-  const float base = m == -INFINITY ? 0.f : m;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  float l = 0.f;
-  for (int k = grp; k < n; k += GROUPS) {
-    const float* s = slot(k);
-    const float f = ex2(s[R * HD + 2 * r] - base);
-    const float4 v = reinterpret_cast<const float4*>(s + r * HD)[sub];
-    acc.x = fmaf(v.x, f, acc.x), acc.y = fmaf(v.y, f, acc.y), acc.z = fmaf(v.z, f, acc.z), acc.w = fmaf(v.w, f, acc.w);
-    l = fmaf(s[R * HD + 2 * r + 1], f, l);
-  }
-  if (GROUPS > 1) {
-    acc_s[team][sub] = acc;
-    if (sub == 0) l_s[team] = l;
-    __syncthreads();
-    if (grp != 0) return;
-    for (int k = 1; k < GROUPS; ++k) {
-      const float4 v = acc_s[team + k][sub];
-      acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
-      l += l_s[team + k];
-    }
-  }
-  if (!live) return;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  const float x[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+  const int lane = threadIdx.x & 31, team = threadIdx.x >> 5;
+  for_pieces<R>(p, n_cta, [&](const Spanning& b, int c, int r) {
+    if (r >= b.rows) return;
+    const int n = b.last - c + 1;
+    auto slot = [&](int k) { return p.part + (int64_t)(2 * (c + k) + (k == 0 ? 1 : 0)) * (R * (HD + 2)); };
+    float acc[D] = {}, l = 0.f, m = -INFINITY;
+#pragma unroll 4
+    for (int k = team; k < n; k += 8) {
+      const float* s = slot(k);
+      float x[D];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) store_out(p, it.q, it.row_lo + r, begun.y, 4 * sub + i, HD, l == 0.f ? 0.f : x[i]);
-  if (sub == 0) store_lse(p, it.q, it.row_lo + r, begun.y, m, l);
+      for (int i = 0; i < D; ++i) x[i] = s[r * HD + 32 * i + lane];
+      const float mk = s[R * HD + 2 * r], lk = s[R * HD + 2 * r + 1], to = fmaxf(m, mk), base = to == -INFINITY ? 0.f : to;
+      const float f0 = ex2(m - base), f1 = ex2(mk - base);
+      m = to;
+      l = l * f0 + lk * f1;
+#pragma unroll
+      for (int i = 0; i < D; ++i) acc[i] = acc[i] * f0 + x[i] * f1;
+    }
+#pragma unroll
+    for (int i = 0; i < D; ++i) acc_s[team][32 * i + lane] = acc[i];
+    if (lane == 0) m_s[team] = m, l_s[team] = l;
+    __syncthreads();
+    if (threadIdx.x < HD) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) top = fmaxf(top, m_s[k]);
+      const float base = top == -INFINITY ? 0.f : top;
+      float a = 0.f, sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float f = ex2(m_s[k] - base);
+        a = fmaf(acc_s[k][threadIdx.x], f, a);
+        sum = fmaf(l_s[k], f, sum);
+      }
+      store_out(p, b.row0, b.row_lo + r, b.head, threadIdx.x, HD, sum == 0.f ? 0.f : a / sum);
+      if (threadIdx.x == 0) store_lse(p, b.row0, b.row_lo + r, b.head, top, sum);
+    }
+    __syncthreads();
+  });
+}
+
+// Row tiles, triples [d][row]: a piece is 32 rows, a lane a row, by 16 columns.
+template <int HD, int R>
+__global__ void __launch_bounds__(256) kv_combine_tiles_kernel(const __grid_constant__ AttnParams p, int n_cta) {
+  constexpr int D = 16, PD = HD / D;
+  __shared__ float acc_s[8][D][33];
+  __shared__ float m_s[8][32], l_s[8][32];
+  pdl_wait();
+  const int lane = threadIdx.x & 31, team = threadIdx.x >> 5;
+  for_pieces<R / 32 * PD>(p, n_cta, [&](const Spanning& b, int c, int piece) {
+    const int r0 = piece / PD * 32, d0 = piece % PD * D;
+    if (r0 >= b.rows) return;
+    const int n = b.last - c + 1, r = min(r0 + lane, b.rows - 1);
+    auto slot = [&](int k) { return p.part + (int64_t)(2 * (c + k) + (k == 0 ? 1 : 0)) * (R * (HD + 2)) + r; };
+    float acc[D] = {}, l = 0.f, m = -INFINITY;
+    for (int k = team; k < n; k += 8) {
+      const float* s = slot(k);
+      float x[D];
+#pragma unroll
+      for (int i = 0; i < D; ++i) x[i] = s[(d0 + i) * R];
+      const float mk = s[HD * R], lk = s[(HD + 1) * R], to = fmaxf(m, mk), base = to == -INFINITY ? 0.f : to;
+      const float f0 = ex2(m - base), f1 = ex2(mk - base);
+      m = to;
+      l = l * f0 + lk * f1;
+#pragma unroll
+      for (int i = 0; i < D; ++i) acc[i] = acc[i] * f0 + x[i] * f1;
+    }
+#pragma unroll
+    for (int i = 0; i < D; ++i) acc_s[team][i][lane] = acc[i];
+    m_s[team][lane] = m, l_s[team][lane] = l;
+    __syncthreads();
+    // thread: row tid / 8, columns 2 (tid % 8) and the next
+    const int row = threadIdx.x / 8, d = 2 * (threadIdx.x % 8);
+    float top = -INFINITY, x = 0.f, y = 0.f, sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) top = fmaxf(top, m_s[k][row]);
+    const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float f = ex2(m_s[k][row] - base);
+      x = fmaf(acc_s[k][d][row], f, x);
+      y = fmaf(acc_s[k][d + 1][row], f, y);
+      sum = fmaf(l_s[k][row], f, sum);
+    }
+    if (r0 + row < b.rows) {
+      store_out(p, b.row0, b.row_lo + r0 + row, b.head, d0 + d, HD, sum == 0.f ? 0.f : x / sum);
+      store_out(p, b.row0, b.row_lo + r0 + row, b.head, d0 + d + 1, HD, sum == 0.f ? 0.f : y / sum);
+      if (d0 == 0 && d == 0) store_lse(p, b.row0, b.row_lo + r0 + row, b.head, top, sum);
+    }
+    __syncthreads();
+  });
 }
 
 // ---------------------------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------------------------
-constexpr int kRowsGrid = 148;
-constexpr int kTileGrid = 148;
-constexpr int kMaxGrid = 148;
+constexpr int kRowsGrid = kMaxGrid;
+constexpr int kTileGrid = kMaxGrid;
+constexpr int kCombineGrid = 8 * kMaxGrid;
 constexpr int kRowsMax = 16;  // rows of a sequence and key/value head that the few-rows kernel takes
 
 template <int HD, int KV, int NT>
@@ -1289,7 +1397,7 @@ cudaError_t launch_rows(AttnParams p, int max_rows, cudaStream_t st) {
   set_pdl_for_call(true);
   e = launch_pdl(kv_rows_kernel<HD, KV, NT>, dim3(kRowsGrid), dim3(256), C::kSmem, st, p);
   if (e != cudaSuccess) return e;
-  e = launch_pdl(kv_combine_kernel<HD, C::R, C::TILE, 8>, dim3(kRowsGrid, C::R), dim3(8 * HD / 4), 0, st, p);
+  e = launch_pdl(kv_combine_kernel<HD, C::R>, dim3(kCombineGrid), dim3(256), 0, st, p, kRowsGrid);
   set_pdl_for_call(false);
   return e;
 }
@@ -1304,7 +1412,7 @@ cudaError_t launch_tiles(AttnParams p, int max_rows, cudaStream_t st) {
   set_pdl_for_call(true);
   e = launch_pdl(kv_tile_kernel<HD, KV>, dim3(kTileGrid), dim3(C::kThreads), C::kSmem, st, p);
   if (e != cudaSuccess) return e;
-  e = launch_pdl(kv_combine_kernel<HD, C::R, C::TILE, 1>, dim3(kTileGrid, C::R / 8), dim3(8 * HD / 4), 0, st, p);
+  e = launch_pdl(kv_combine_tiles_kernel<HD, C::R>, dim3(kCombineGrid), dim3(256), 0, st, p, kTileGrid);
   set_pdl_for_call(false);
   return e;
 }
@@ -1317,7 +1425,7 @@ cudaError_t launch_kv(const AttnParams& p, int max_rows, cudaStream_t st) {
 }
 
 // desc, the waits' error word, partial triples (two a CTA) of the larger row tile that max_rows can need
-constexpr size_t kWsHead = kMaxGrid * sizeof(int4) + 16;
+constexpr size_t kWsHead = kMaxGrid * sizeof(Spanning) + 16;
 size_t workspace_bytes_of(int hd, int64_t max_rows) {
   const int64_t rows = max_rows <= kRowsMax ? kRowsMax : 256;
   return kWsHead + (size_t)kMaxGrid * 2 * rows * (hd + 2) * 4;
@@ -1385,7 +1493,7 @@ extern "C" dmoe_status dmoe_kv_attention(const dmoe_kv_cache* cache, const dmoe_
   p.vec_q16 = ((reinterpret_cast<uintptr_t>(a->q) | (uintptr_t)(2 * a->q_stride)) & 15u) == 0;
   p.vec_out16 = ((reinterpret_cast<uintptr_t>(a->out) | (uintptr_t)(2 * a->out_stride)) & 15u) == 0;
   p.scale_log2 = a->scale * kLog2e;
-  p.desc = static_cast<int4*>(workspace);
+  p.desc = static_cast<Spanning*>(workspace);
   p.wait_err = cache->err ? cache->err : reinterpret_cast<uint32_t*>(p.desc + kMaxGrid);
   p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kWsHead);
   const int max_rows = (int)max_rows_of(cache, batch, a);
