@@ -65,9 +65,10 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// the largest of three, NaN if one is
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
 
@@ -87,6 +88,26 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
+}
+
+// 2^t of two numbers on the FMA and integer pipes: t = n + f with n the nearest integer, 2^f = 1 + f q(f) on
+// [-1/2, 1/2] with q the cubic of least relative error there (2.9e-6, from a weighted least-squares fit), and n
+// added to the exponent field. t is cut at -127, where f = 0 and the result is exactly 0.
+__device__ __forceinline__ void ex2_fma(uint64_t t, float& a, float& b) {
+  unpair(t, a, b);
+  t = pair(fmaxf(a, -127.f), fmaxf(b, -127.f));
+  const uint64_t magic = pair(12582912.f, 12582912.f);  // 1.5 * 2^23: the sum's low bits are n
+  const uint64_t r = add2(t, magic);
+  const uint64_t f = fma2(add2(r, pair(-12582912.f, -12582912.f)), pair(-1.f, -1.f), t);
+  uint64_t q = fma2(f, pair(0x1.3a02dp-7f, 0x1.3a02dp-7f), pair(0x1.c9fc48p-5f, 0x1.c9fc48p-5f));
+  q = fma2(f, q, pair(0x1.ec0378p-3f, 0x1.ec0378p-3f));
+  q = fma2(f, q, pair(0x1.62e12cp-1f, 0x1.62e12cp-1f));
+  q = fma2(f, q, pair(1.f, 1.f));
+  float r0, r1, q0, q1;
+  unpair(r, r0, r1);
+  unpair(q, q0, q1);
+  a = __int_as_float(__float_as_int(q0) + (__float_as_int(r0) << 23));
+  b = __int_as_float(__float_as_int(q1) + (__float_as_int(r1) << 23));
 }
 
 // 2^e for |e| <= 126
@@ -121,56 +142,57 @@ __device__ __forceinline__ Item item_of(const AttnParams& p, int u) {
 
 // Beginning and ending an item costs about as much as OV tiles. An item of t tiles is OV + t units long, and
 // the units of all items are numbered through; its tiles are the last t.
-struct Run {       // a CTA's run of units
-  Item it;         // first item
+// The host refuses calls whose units could number 2^31 or more.
+struct Run {   // a CTA's run of units
+  Item it;     // first item
   int u, head;
-  int unit;        // first unit within it
-  int left;        // units of the run (2^31 tiles would take an hour: no workload has them)
-  int chunk;       // units of every run but the last
-  int64_t first;   // number of the first unit
+  int unit;    // first unit within it
+  int left;    // units of the run
+  int chunk;   // units of every run but the last
+  int first;   // number of the first unit
 };
 
-// The whole CTA: finds its run. smem: scratch of THREADS / 32 + 1 words and one Run.
+// The whole CTA: finds its run. sums: THREADS / 32 words of shared memory.
 template <int R, int TILE, int OV, int THREADS>
-__device__ __forceinline__ Run find_run(const AttnParams& p, int64_t* sums, Run* found) {
+__device__ __forceinline__ Run find_run(const AttnParams& p, int* sums, Run* found) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int64_t n_u = (int64_t)p.b.n_seq * p.n_qt;
-  const int64_t per = (n_u + THREADS - 1) / THREADS;
-  const int64_t u0 = min(n_u, per * tid), u1 = min(n_u, u0 + per);
-  int64_t mine = 0;
-  for (int64_t u = u0; u < u1; ++u) {
-    const int t = item_of<R, TILE>(p, (int)u).tiles;
+  const int n_u = p.b.n_seq * p.n_qt;
+  const int per = (n_u + THREADS - 1) / THREADS;
+  const int u0 = min((int64_t)n_u, (int64_t)per * tid), u1 = min((int64_t)n_u, (int64_t)u0 + per);
+  int mine = 0;
+  for (int u = u0; u < u1; ++u) {
+    const int t = item_of<R, TILE>(p, u).tiles;
     if (t) mine += t + OV;
   }
-  int64_t incl = mine;
+  int incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+    const int v = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += v;
   }
   if (lane == 31) sums[warp] = incl;
   if (tid == 0) found->left = 0;
   __syncthreads();
-  int64_t before = incl - mine, total = 0;
+  int before = incl - mine, total = 0;
   for (int w = 0; w < THREADS / 32; ++w) {
     if (w < warp) before += sums[w];
     total += sums[w];
   }
   const int heads = p.pg.n_head_kv;
   total *= heads;
-  const int64_t chunk = min((total + gridDim.x - 1) / gridDim.x, (int64_t)INT32_MAX);
-  const int64_t first = chunk * blockIdx.x;
+  const int chunk = (int)(((uint32_t)total + gridDim.x - 1) / gridDim.x);
+  const int first = (int)min((int64_t)chunk * blockIdx.x, (int64_t)total);
   before *= heads;
   if (first < total && first >= before && first < before + mine * heads) {
-    for (int64_t u = u0; u < u1; ++u) {
-      const Item it = item_of<R, TILE>(p, (int)u);
-      const int64_t w = it.tiles ? it.tiles + OV : 0;
+    for (int u = u0; u < u1; ++u) {
+      const Item it = item_of<R, TILE>(p, u);
+      const int w = it.tiles ? it.tiles + OV : 0;
       if (first < before + w * heads) {
         found->it = it;
-        found->u = (int)u;
-        found->head = (int)((first - before) / w);
-        found->unit = (int)((first - before) % w);
-        found->left = (int)min(chunk, total - first);
+        found->u = u;
+        found->head = (first - before) / w;
+        found->unit = (first - before) % w;
+        found->left = min(chunk, total - first);
         break;
       }
       before += w * heads;
@@ -178,7 +200,7 @@ __device__ __forceinline__ Run find_run(const AttnParams& p, int64_t* sums, Run*
   }
   __syncthreads();
   Run r = *found;
-  r.chunk = (int)chunk;
+  r.chunk = chunk;
   r.first = first;
   return r;
 }
@@ -190,8 +212,7 @@ struct Walk {
   const AttnParams& p;
   Item it;
   int u, head, seg = -1, t0 = 0, t1 = 0;
-  int unit, left, chunk;
-  int64_t at;
+  int unit, left, chunk, at;
   __device__ __forceinline__ Walk(const AttnParams& p_, const Run& r)
       : p(p_), it(r.it), u(r.u), head(r.head), unit(r.unit), left(r.left), chunk(r.chunk), at(r.first) {
     settle();
@@ -200,7 +221,7 @@ struct Walk {
   __device__ __forceinline__ bool whole() const { return t0 == 0 && t1 == it.tiles; }
   // for an item that this CTA begins and does not end
   __device__ __forceinline__ Spanning begun() const {
-    return {(int)((at - unit + OV + it.tiles - 1) / chunk), it.q.row0, it.row_lo, it.rows, head, {0, 0, 0}};
+    return {(at - unit + OV + it.tiles - 1) / chunk, it.q.row0, it.row_lo, it.rows, head, {0, 0, 0}};
   }
   __device__ __forceinline__ void next() {
     advance();
@@ -222,7 +243,7 @@ struct Walk {
   __device__ __forceinline__ void settle() {
     while (left > 0) {
       t0 = max(0, unit - OV);
-      t1 = (int)min((int64_t)it.tiles, (int64_t)unit + left - OV);
+      t1 = min(it.tiles, unit + left - OV);
       if (t1 > t0) break;
       advance();
     }
@@ -359,7 +380,7 @@ __global__ void __launch_bounds__(256, 1) kv_rows_kernel(const __grid_constant__
   constexpr int VW = VB / 4;
   constexpr int JT = HD / 16;              // 16-row tiles of o^T
   extern __shared__ float smem_f[];
-  __shared__ int64_t sums[C::kWarps];
+  __shared__ int sums[C::kWarps];
   __shared__ Run found;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
 
@@ -506,12 +527,19 @@ __global__ void __launch_bounds__(256, 1) kv_rows_kernel(const __grid_constant__
 #pragma unroll
         for (int a = 0; a < MT; ++a)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float x = fmaf(s[n][a][i], cq[n][i & 1] * sk, evf);
-            if (edge && here + 16 * a + 8 * (i >> 1) + g >= lim[n][i & 1]) x = -INFINITY;
-            s[n][a][i] = x;
-            mx[i & 1] = fmaxf(mx[i & 1], x);
-          }
+          for (int i = 0; i < 4; ++i) s[n][a][i] = fmaf(s[n][a][i], cq[n][i & 1] * sk, evf);
+        if (edge) {
+          asm volatile("" ::: "memory");  // stay a branch
+#pragma unroll
+          for (int a = 0; a < MT; ++a)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (here + 16 * a + 8 * (i >> 1) + g >= lim[n][i & 1]) s[n][a][i] = -INFINITY;
+        }
+#pragma unroll
+        for (int a = 0; a < MT; ++a)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mx[i & 1] = fmaxf(mx[i & 1], s[n][a][i]);
         float base[2], shrink[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -689,6 +717,7 @@ struct TileCfg {
   static constexpr int OV = 2;
   static constexpr int kThreads = 640, kLoaders = 128;
   // registers a thread: 256 * 160 + 256 * 64 + 128 * 32 = the 640 * 96 of the launch
+  static constexpr int kFmaPairs = 0;  // of 8 pairs of exponentials, those off the exponential unit
   static constexpr int kSoftmaxRegs = 160, kLoadRegs = 64, kIssueRegs = 32;
   static constexpr int kPlane = 128 * 128;             // 64 elements of 128 rows
   static constexpr int kOperand = HD / 64 * kPlane;    // bytes of a 128-row operand
@@ -717,13 +746,13 @@ __global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__
   extern __shared__ uint8_t smem_raw[];
   __shared__ TileBars bar;
   __shared__ uint32_t tmem_base_s;
-  __shared__ int64_t sums[C::kThreads / 32];
+  __shared__ int sums[C::kThreads / 32];
   __shared__ Run found;
   __shared__ int not_finite_from[4][HD];  // [item of the run & 3][d]: first position whose value is not finite
   __shared__ int any_not_finite[4];
-  // scale exponents [value][tile of the run & 3][32-position block]. Written before the tile's arrival; the
+  // scales of keys, exponents of values and their reciprocal scales [..][tile of the run & 3][32-position block]. Written before the tile's arrival; the
   // slot is free again when the tile two on has been multiplied by both halves' queries
-  __shared__ int scale_s[2][4][4];
+  __shared__ __align__(16) float scale_s[3][4][4];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* q_s = smem;                                 // [half] operands
   uint8_t* k_s = q_s + 2 * C::kOperand;                // [stage]
@@ -846,7 +875,8 @@ __global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__
     bool ok = true;
     // first row of each of the tile's 32-position blocks in the pages. The page numbers of eight tiles
     // are read at once, one a lane
-    int64_t first_row[4];
+    const uint8_t* block_at[4];  // this thread's piece of its first row in each block
+    int64_t scale_at = 0;         // scale of block `lane` of the tile (lanes 0-3)
     int held = 0, held_from = 0;  // blocks [held_from, held_from + 32) of the item
     auto get_pages = [&](int tile, int lim, bool new_item) {
       const int b0 = tile * (TILE / 32);
@@ -865,11 +895,13 @@ __global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__
       for (int i = 0; i < 4; ++i) {
         const int page = __shfl_sync(0xffffffffu, held, b0 + i - held_from);
         const uint32_t b = b0 + i;
-        first_row[i] = kv_row(p.pg, page, w.head, (int)(b - kv_slot(p.pg, b) * p.pg.page_blocks) * kScaleBlock);
+        const int64_t blk = ((int64_t)page * p.pg.n_head_kv + w.head) * p.pg.page_blocks + (b - kv_slot(p.pg, b) * p.pg.page_blocks);
+        block_at[i] = base + blk * (32 * HD * ES) + r0 * (HD * ES) + 16 * c;
+        if (KV == KV_E4M3 && lane == i) scale_at = blk;
       }
     };
     // this thread's i-th piece of the tile; its row is r0 + i * RPI
-    auto source = [&](int i) { return base + (first_row[i * RPI / 32] + ((r0 + i * RPI) & 31)) * (HD * ES) + 16 * c; };
+    auto source = [&](int i) { return block_at[i * RPI / 32] + (i * RPI % 32) * (HD * ES); };
     // Values at positions that only some rows see, where they are not finite: their products with a zero
     // weight would reach the other rows. They are set to zero, and their element marked for the rows that see them
     auto mark = [&](int seg, int pos, int d) {
@@ -890,14 +922,16 @@ __global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__
     auto fetch = [&](int tile, int lim) {
       if constexpr (KV == KV_E4M3) {
         scale = 0;
-        if (lt < 4 && tile * TILE + 32 * lt < lim) {
-          const int64_t row = lt == 0 ? first_row[0] : lt == 1 ? first_row[1] : lt == 2 ? first_row[2] : first_row[3];
-          scale = (int)(is_v ? p.pg.v_scale : p.pg.k_scale)[row / kScaleBlock] - 127;
-        }
+        if (lt < 4 && tile * TILE + 32 * lt < lim) scale = (int)(is_v ? p.pg.v_scale : p.pg.k_scale)[scale_at] - 127;
+        if ((tile + 1) * TILE <= lim) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          x[i] = make_uint4(0, 0, 0, 0);
-          if (tile * TILE + r0 + i * RPI < lim) x[i] = __ldg(reinterpret_cast<const uint4*>(source(i)));
+          for (int i = 0; i < N; ++i) x[i] = __ldg(reinterpret_cast<const uint4*>(source(i)));
+        } else {
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            x[i] = make_uint4(0, 0, 0, 0);
+            if (tile * TILE + r0 + i * RPI < lim) x[i] = __ldg(reinterpret_cast<const uint4*>(source(i)));
+          }
         }
       }
     };
@@ -918,7 +952,12 @@ __global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__
         if (!ok) break;
         const bool edge = is_v && lim_min < lim_max && (t + 1) * TILE > lim_min;
         if constexpr (KV == KV_E4M3) {
-          if (lt < 4) *const_cast<volatile int*>(&scale_s[is_v][n & 3][lt]) = scale;
+          if (lt < 4) {
+            if (is_v)
+              scale_s[1][n & 3][lt] = (float)scale, scale_s[2][n & 3][lt] = pow2i(-scale);
+            else
+              scale_s[0][n & 3][lt] = pow2i(scale);
+          }
           if (edge) {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
@@ -955,12 +994,19 @@ __global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__
           // 16-bit pages need no conversion
           uint8_t* const mine = dst + (c / 8) * C::kPlane + r0 * 128 + 16 * ((c % 8) ^ (r0 & 7));
           static_assert(RPI % 8 == 0, "the swizzle of a thread's rows is one");
+          const uint32_t to = smem_u32(mine);
+          if ((t + 1) * TILE <= lim_max) {
 #pragma unroll
-          for (int i = 0; i < N; ++i) {
-            const bool in = t * TILE + r0 + i * RPI < lim_max;
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(mine + i * RPI * 128)),
-                         "l"(in ? source(i) : base), "r"(in ? 16 : 0)
-                         : "memory");
+            for (int i = 0; i < N; ++i)
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + i * RPI * 128), "l"(source(i)) : "memory");
+          } else {
+#pragma unroll 4
+            for (int i = 0; i < N; ++i) {
+              const bool in = t * TILE + r0 + i * RPI < lim_max;
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + i * RPI * 128), "l"(in ? source(i) : base),
+                           "r"(in ? 16 : 0)
+                           : "memory");
+            }
           }
           asm volatile("cp.async.wait_all;" ::: "memory");
           if (edge) {
@@ -1093,35 +1139,53 @@ __global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__
         if (!ok) break;
         ph_s ^= 1;
         tc_fence_after();
-        uint32_t x[4][32];
+        // 32 scores at a time, the next ones on their way; they are read twice, since a row of 128 in registers
+        // leaves none to overlap the exponentials with
+        uint32_t x[2][32];
+        tmem_ld32(s_addr, x[0]);
+        float c[4], ev[4], un[4];  // score factors, exponents of the values' scales, their reciprocals
+        if (KV == KV_E4M3) {
+          const float4 k = *reinterpret_cast<const float4*>(scale_s[0][n & 3]), v = *reinterpret_cast<const float4*>(scale_s[1][n & 3]),
+                       u = *reinterpret_cast<const float4*>(scale_s[2][n & 3]);
+          c[0] = factor * k.x, c[1] = factor * k.y, c[2] = factor * k.z, c[3] = factor * k.w;
+          ev[0] = v.x, ev[1] = v.y, ev[2] = v.z, ev[3] = v.w;
+          un[0] = u.x, un[1] = u.y, un[2] = u.z, un[3] = u.w;
+        } else {
 #pragma unroll
-        for (int b = 0; b < 4; ++b) tmem_ld32(s_addr + 32 * b, x[b]);
-        float c[4], ev[4];
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          c[b] = KV == KV_E4M3 ? factor * pow2i(*const_cast<volatile int*>(&scale_s[0][n & 3][b])) : factor;
-          ev[b] = KV == KV_E4M3 ? (float)*const_cast<volatile int*>(&scale_s[1][n & 3][b]) : 0.f;
+          for (int b = 0; b < 4; ++b) c[b] = factor, ev[b] = 0.f, un[b] = 1.f;
         }
-        tmem_wait_ld();
-        if ((t + 1) * TILE > lim_warp) {
-          const int valid = lim - t * TILE;  // columns this row sees
-#pragma unroll
-          for (int b = 0; b < 4; ++b)
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (32 * b + i >= valid) x[b][i] = 0xff800000u;
-        }
+        const bool edge = (t + 1) * TILE > lim_warp;
+        const int valid = lim - t * TILE;  // columns this row sees
         float mx = -INFINITY;
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-          float top[2] = {__uint_as_float(x[b][0]), __uint_as_float(x[b][1])};
+          uint32_t(&y)[32] = x[b & 1];
+          tmem_wait_ld();
+          if (b < 3) tmem_ld32(s_addr + 32 * (b + 1), x[(b + 1) & 1]);
+          if (edge) {  // scores that the row does not see, here and (a store keeps this a branch) in TMEM
 #pragma unroll
-          for (int i = 2; i < 30; i += 4) {
-            top[0] = max3(top[0], __uint_as_float(x[b][i]), __uint_as_float(x[b][i + 1]));
-            top[1] = max3(top[1], __uint_as_float(x[b][i + 2]), __uint_as_float(x[b][i + 3]));
+            for (int i = 0; i < 32; ++i) y[i] = 32 * b + i < valid ? y[i] : 0xff800000u;
+            tmem_st16(s_addr + 32 * b, reinterpret_cast<uint32_t(&)[16]>(y[0]));
+            tmem_st16(s_addr + 32 * b + 16, reinterpret_cast<uint32_t(&)[16]>(y[16]));
           }
-          top[0] = max3(top[0], __uint_as_float(x[b][30]), __uint_as_float(x[b][31]));
-          mx = fmaxf(mx, fmaf(fmaxf(top[0], top[1]), c[b], ev[b]));
+          float top[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) top[i] = max3(__uint_as_float(y[8 * i]), __uint_as_float(y[8 * i + 1]), __uint_as_float(y[8 * i + 2]));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) top[i] = max3(top[i], __uint_as_float(y[8 * i + 3]), __uint_as_float(y[8 * i + 4]));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) top[i] = max3(top[i], __uint_as_float(y[8 * i + 5]), __uint_as_float(y[8 * i + 6]));
+          top[0] = max3(top[0], __uint_as_float(y[7]), top[1]);
+          top[2] = max3(top[2], __uint_as_float(y[15]), top[3]);
+          top[0] = max3(top[0], __uint_as_float(y[23]), top[2]);
+          top[0] = max3(top[0], __uint_as_float(y[31]), top[0]);
+          mx = max3(mx, fmaf(top[0], c[b], ev[b]), mx);
+        }
+        if (edge) tmem_wait_st();
+        tmem_ld32(s_addr, x[0]);
+        if (!(mx < INFINITY)) {  // a score that is NaN or infinite: so is the row, whatever the weights become
+          l = __int_as_float(0x7fc00000);
+          mx = m;
         }
         float shrink = 1.f;
         if (mx > m + 8.f || m == -INFINITY) {
@@ -1145,21 +1209,29 @@ __global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__
         const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
+          uint32_t(&y)[32] = x[b & 1];
+          tmem_wait_ld();
+          if (b < 3) tmem_ld32(s_addr + 32 * (b + 1), x[(b + 1) & 1]);
           const uint64_t c2 = pair(c[b], c[b]), off2 = pair(ev[b] - base, ev[b] - base);
-          uint64_t sum = pair(0.f, 0.f);
+          uint64_t sum[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
           uint32_t pk[16];
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
             float a, d;
-            unpair(fma2(pair(__uint_as_float(x[b][i]), __uint_as_float(x[b][i + 1])), c2, off2), a, d);
-            a = ex2(a), d = ex2(d);
-            sum = add2(sum, pair(a, d));
+            const uint64_t e = fma2(pair(__uint_as_float(y[i]), __uint_as_float(y[i + 1])), c2, off2);
+            if (i / 2 % 8 < C::kFmaPairs) {
+              ex2_fma(e, a, d);
+            } else {
+              unpair(e, a, d);
+              a = ex2(a), d = ex2(d);
+            }
+            sum[i / 2 & 1] = add2(sum[i / 2 & 1], pair(a, d));
             pk[i / 2] = pack2<kBf>(a, d);
           }
           tmem_st16(s_addr + 16 * b, pk);
           float a, d;
-          unpair(sum, a, d);
-          l = fmaf(a + d, KV == KV_E4M3 ? pow2i(-(int)ev[b]) : 1.f, l);
+          unpair(add2(sum[0], sum[1]), a, d);
+          l = fmaf(a + d, un[b], l);
         }
         tmem_wait_st();
         tc_fence_before();
@@ -1467,6 +1539,13 @@ extern "C" dmoe_status dmoe_kv_attention(const dmoe_kv_cache* cache, const dmoe_
   const int group = a->n_head / cache->n_head_kv;
   if (((int64_t)std::min<int64_t>(batch->max_q_len, a->n_tokens) * group + 7) * std::max(1, batch->n_seq) > INT32_MAX)
     return fail(DMOE_ERR_UNSUPPORTED, "n_seq * max_q_len * n_head / n_head_kv must be below 2^31");
+  {
+    // units of work, at most: row tiles of 8 or 256 rows, by tiles of 128 positions at least
+    const int64_t rows = max_rows_of(cache, batch, a), tile = rows <= kRowsMax ? 8 : 256;
+    const double items = std::min((double)batch->n_seq * ((rows + tile - 1) / tile), (double)a->n_tokens * group / tile + batch->n_seq);
+    if (items * ((double)batch->max_pages * cache->page_size / 128 + 4) * cache->n_head_kv >= 2147483648.0)
+      return fail(DMOE_ERR_UNSUPPORTED, "rows times positions of the page table too many for one call");
+  }
   if (a->n_tokens == 0 || batch->n_seq == 0 || batch->max_q_len == 0) return DMOE_OK;
   if (!a->q || !a->out || !workspace) return fail(DMOE_ERR_INVALID_ARG, "null pointer");
   if ((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->out)) & 1u ||
