@@ -793,70 +793,65 @@ __global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kIssueRegs));
     Walk<R, TILE, C::OV> w(p, run);
     if (warp == 16) {
-    // ---- products
-    uint32_t kv_n = 0;           // tiles whose keys were used
-    uint32_t ph_p[2] = {0, 0};
-    bool ok = true;
-    const uint32_t k_addr = smem_u32(k_s), v_addr = smem_u32(v_s), q_addr = smem_u32(q_s);
-    auto scores = [&](int half, int stage) {
+      // ---- products: one thread waits and issues, so that nothing but the waits lies between them
       if (elect_one()) {
-        const uint32_t qa = q_addr + half * C::kOperand, ka = k_addr + stage * C::kOperand;
+        uint32_t n = 0;  // tiles whose keys were used
+        uint32_t ph_p[2] = {0, 0};
+        bool ok = true;
+        auto wait = [&](uint64_t* b, uint32_t parity) { return mbar_wait(b, parity, err, kTimeout); };
+        const uint64_t q_desc = sdesc_sw128(smem_u32(q_s), 1024), k_desc = sdesc_sw128(smem_u32(k_s), 1024),
+                       v_desc = sdesc_sw128_mn(smem_u32(v_s), C::kPlane);
+        auto scores = [&](int half, int stage) {
+          const uint64_t qd = q_desc + half * (C::kOperand / 16), kd = k_desc + stage * (C::kOperand / 16);
 #pragma unroll
-        for (int k = 0; k < HD / 16; ++k) {
-          const uint32_t off = (k / 4) * C::kPlane + (k % 4) * 32;
-          mma_f16_ss(tmem + half * 128, sdesc_sw128(qa + off, 1024), sdesc_sw128(ka + off, 1024), kIdescS, k > 0);
-        }
-        mma_commit(&bar.s_full[half]);
-      }
-      __syncwarp();
-    };
-    auto outputs = [&](int half, int stage, bool first) {
-      if (elect_one()) {
-        const uint32_t va = v_addr + stage * C::kOperand;
+          for (int k = 0; k < HD / 16; ++k) {
+            const int off = ((k / 4) * C::kPlane + (k % 4) * 32) / 16;
+            mma_f16_ss(tmem + half * 128, qd + off, kd + off, kIdescS, k > 0);
+          }
+          mma_commit(&bar.s_full[half]);
+        };
+        auto outputs = [&](int half, int stage, bool first) {
+          const uint64_t vd = v_desc + stage * (C::kOperand / 16);
+          mma_f16_ts(tmem + 256 + half * 128, tmem + half * 128, vd, kIdescO, !first);
 #pragma unroll
-        for (int k = 0; k < TILE / 16; ++k)
-          mma_f16_ts(tmem + 256 + half * 128, tmem + half * 128 + 8 * k, sdesc_sw128_mn(va + 2048 * k, C::kPlane), kIdescO,
-                     !(first && k == 0));
-      }
-      __syncwarp();
-    };
-    auto commit = [&](uint64_t* b) {
-      if (elect_one()) mma_commit(b);
-      __syncwarp();
-    };
-    for (; ok && w.more(); w.next()) {
-      const int halves = w.it.rows > 128 ? 2 : 1;
-      const int n = w.t1 - w.t0;
-      ok = warp_wait(&bar.q_full, w.seg & 1, err, kTimeout);
-      if (ok) ok = warp_wait(&bar.k_full[kv_n & 1], (kv_n >> 1) & 1, err, kTimeout);
-      if (!ok) break;
-      tc_fence_after();
-      for (int h = 0; h < halves; ++h) scores(h, kv_n & 1);
-      commit(&bar.k_empty[kv_n & 1]);
-      for (int j = 0; ok && j < n; ++j, ++kv_n) {
-        const int stage = kv_n & 1, next = (kv_n + 1) & 1;
-        ok = warp_wait(&bar.v_full[stage], (kv_n >> 1) & 1, err, kTimeout);
-        for (int h = 0; ok && h < halves; ++h) {
-          ok = warp_wait(&bar.p_full[h], ph_p[h], err, kTimeout);
+          for (int k = 1; k < TILE / 16; ++k)
+            mma_f16_ts(tmem + 256 + half * 128, tmem + half * 128 + 8 * k, vd + k * (2048 / 16), kIdescO, 1);
+        };
+        for (; ok && w.more(); w.next()) {
+          const int halves = w.it.rows > 128 ? 2 : 1, tiles = w.t1 - w.t0;
+          ok = wait(&bar.q_full, w.seg & 1) && wait(&bar.k_full[n & 1], (n >> 1) & 1);
           if (!ok) break;
-          ph_p[h] ^= 1;
           tc_fence_after();
-          outputs(h, stage, j == 0);
-          if (h == halves - 1) commit(&bar.v_empty[stage]);
-          if (j + 1 < n) {
-            if (h == 0) ok = warp_wait(&bar.k_full[next], ((kv_n + 1) >> 1) & 1, err, kTimeout);
-            if (!ok) break;
-            tc_fence_after();
-            scores(h, next);
-            if (h == halves - 1) commit(&bar.k_empty[next]);
-          } else {
-            commit(&bar.o_full[h]);
+          for (int h = 0; h < halves; ++h) scores(h, n & 1);
+          mma_commit(&bar.k_empty[n & 1]);
+          for (int j = 0; ok && j < tiles; ++j, ++n) {
+            const int stage = n & 1, next = (n + 1) & 1;
+            ok = wait(&bar.v_full[stage], (n >> 1) & 1);
+            for (int h = 0; ok && h < halves; ++h) {
+              ok = wait(&bar.p_full[h], ph_p[h]);
+              if (!ok) break;
+              ph_p[h] ^= 1;
+              tc_fence_after();
+              outputs(h, stage, j == 0);
+              if (h == halves - 1) mma_commit(&bar.v_empty[stage]);
+              if (j + 1 < tiles) {
+                if (h == 0) {
+                  ok = wait(&bar.k_full[next], ((n + 1) >> 1) & 1);
+                  if (!ok) break;
+                  tc_fence_after();
+                }
+                scores(h, next);
+                if (h == halves - 1) mma_commit(&bar.k_empty[next]);
+              } else {
+                mma_commit(&bar.o_full[h]);
+              }
+            }
           }
         }
+        mma_commit(&bar.done);  // every product that was issued has ended before TMEM is freed
+        wait(&bar.done, 0);
       }
-    }
-    commit(&bar.done);  // every product that was issued has ended before TMEM is freed
-    warp_wait(&bar.done, 0, err, kTimeout);
+      __syncwarp();
     }
   } else if (warp >= 8) {
     // ---- keys (warps 8-11) and values (12-15)
