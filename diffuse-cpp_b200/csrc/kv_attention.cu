@@ -90,26 +90,6 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   return r;
 }
 
-// 2^t of two numbers on the FMA and integer pipes: t = n + f with n the nearest integer, 2^f = 1 + f q(f) on
-// [-1/2, 1/2] with q the cubic of least relative error there (2.9e-6, from a weighted least-squares fit), and n
-// added to the exponent field. t is cut at -127, where f = 0 and the result is exactly 0.
-__device__ __forceinline__ void ex2_fma(uint64_t t, float& a, float& b) {
-  unpair(t, a, b);
-  t = pair(fmaxf(a, -127.f), fmaxf(b, -127.f));
-  const uint64_t magic = pair(12582912.f, 12582912.f);  // 1.5 * 2^23: the sum's low bits are n
-  const uint64_t r = add2(t, magic);
-  const uint64_t f = fma2(add2(r, pair(-12582912.f, -12582912.f)), pair(-1.f, -1.f), t);
-  uint64_t q = fma2(f, pair(0x1.3a02dp-7f, 0x1.3a02dp-7f), pair(0x1.c9fc48p-5f, 0x1.c9fc48p-5f));
-  q = fma2(f, q, pair(0x1.ec0378p-3f, 0x1.ec0378p-3f));
-  q = fma2(f, q, pair(0x1.62e12cp-1f, 0x1.62e12cp-1f));
-  q = fma2(f, q, pair(1.f, 1.f));
-  float r0, r1, q0, q1;
-  unpair(r, r0, r1);
-  unpair(q, q0, q1);
-  a = __int_as_float(__float_as_int(q0) + (__float_as_int(r0) << 23));
-  b = __int_as_float(__float_as_int(q1) + (__float_as_int(r1) << 23));
-}
-
 // 2^e for |e| <= 126
 __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }
 
@@ -717,7 +697,6 @@ struct TileCfg {
   static constexpr int OV = 2;
   static constexpr int kThreads = 640, kLoaders = 128;
   // registers a thread: 256 * 160 + 256 * 64 + 128 * 32 = the 640 * 96 of the launch
-  static constexpr int kFmaPairs = 0;  // of 8 pairs of exponentials, those off the exponential unit
   static constexpr int kSoftmaxRegs = 160, kLoadRegs = 64, kIssueRegs = 32;
   static constexpr int kPlane = 128 * 128;             // 64 elements of 128 rows
   static constexpr int kOperand = HD / 64 * kPlane;    // bytes of a 128-row operand
@@ -1214,12 +1193,8 @@ __global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__
           for (int i = 0; i < 32; i += 2) {
             float a, d;
             const uint64_t e = fma2(pair(__uint_as_float(y[i]), __uint_as_float(y[i + 1])), c2, off2);
-            if (i / 2 % 8 < C::kFmaPairs) {
-              ex2_fma(e, a, d);
-            } else {
-              unpair(e, a, d);
-              a = ex2(a), d = ex2(d);
-            }
+            unpair(e, a, d);
+            a = ex2(a), d = ex2(d);
             sum[i / 2 & 1] = add2(sum[i / 2 & 1], pair(a, d));
             pk[i / 2] = pack2<kBf>(a, d);
           }
@@ -1342,7 +1317,20 @@ __device__ __forceinline__ void for_pieces(const AttnParams& p, int n_cta, F&& f
     from_s[i] = tid;
   }
   __syncthreads();
-  for (int i = blockIdx.x; i < total * PIECES; i += gridDim.x) f(begun_s[i / PIECES], from_s[i / PIECES], i % PIECES);
+  for (int i = blockIdx.x; i < total * PIECES; i += gridDim.x) {
+    const int piece = i / total, at = i - piece * total;  // first pieces first: an item may have fewer
+    f(begun_s[at], from_s[at], piece);
+  }
+}
+
+// Adds triple (mk, lk, x) to (m, l, acc).
+template <int D>
+__device__ __forceinline__ void join(float& m, float& l, float (&acc)[D], float mk, float lk, const float (&x)[D]) {
+  const float to = fmaxf(m, mk), base = to == -INFINITY ? 0.f : to, f0 = ex2(m - base), f1 = ex2(mk - base);
+  m = to;
+  l = l * f0 + lk * f1;
+#pragma unroll
+  for (int i = 0; i < D; ++i) acc[i] = acc[i] * f0 + x[i] * f1;
 }
 
 // Few rows, triples [row][d]: a piece is a row.
@@ -1364,12 +1352,7 @@ __global__ void __launch_bounds__(256) kv_combine_kernel(const __grid_constant__
       float x[D];
 #pragma unroll
       for (int i = 0; i < D; ++i) x[i] = s[r * HD + 32 * i + lane];
-      const float mk = s[R * HD + 2 * r], lk = s[R * HD + 2 * r + 1], to = fmaxf(m, mk), base = to == -INFINITY ? 0.f : to;
-      const float f0 = ex2(m - base), f1 = ex2(mk - base);
-      m = to;
-      l = l * f0 + lk * f1;
-#pragma unroll
-      for (int i = 0; i < D; ++i) acc[i] = acc[i] * f0 + x[i] * f1;
+      join(m, l, acc, s[R * HD + 2 * r], s[R * HD + 2 * r + 1], x);
     }
 #pragma unroll
     for (int i = 0; i < D; ++i) acc_s[team][32 * i + lane] = acc[i];
@@ -1394,31 +1377,66 @@ __global__ void __launch_bounds__(256) kv_combine_kernel(const __grid_constant__
   });
 }
 
-// Row tiles, triples [d][row]: a piece is 32 rows, a lane a row, by 16 columns.
+// Row tiles, triples [d][row]. Up to 8 triples: a piece is 32 rows, a lane a row and a warp an eighth of the
+// columns, all triples' loads on their way at once. More (a few items over the whole GPU): a piece is 32 rows by 16
+// columns and the warps share the triples.
 template <int HD, int R>
 __global__ void __launch_bounds__(256) kv_combine_tiles_kernel(const __grid_constant__ AttnParams p, int n_cta) {
-  constexpr int D = 16, PD = HD / D;
+  constexpr int D = 16, PD = HD / D, DW = HD / 8;
   __shared__ float acc_s[8][D][33];
   __shared__ float m_s[8][32], l_s[8][32];
+  uint16_t(*const out_s)[HD + 8] = reinterpret_cast<uint16_t(*)[HD + 8]>(&acc_s[0][0][0]);
+  static_assert(sizeof(acc_s) >= 32 * (HD + 8) * 2, "the output of 32 rows fits");
   pdl_wait();
   const int lane = threadIdx.x & 31, team = threadIdx.x >> 5;
   for_pieces<R / 32 * PD>(p, n_cta, [&](const Spanning& b, int c, int piece) {
-    const int r0 = piece / PD * 32, d0 = piece % PD * D;
+    const int n = b.last - c + 1;
+    const bool few = n <= 8;
+    const int r0 = (few ? piece : piece / PD) * 32, d0 = few ? 0 : piece % PD * D;
     if (r0 >= b.rows) return;
-    const int n = b.last - c + 1, r = min(r0 + lane, b.rows - 1);
+    const int r = min(r0 + lane, b.rows - 1);
     auto slot = [&](int k) { return p.part + (int64_t)(2 * (c + k) + (k == 0 ? 1 : 0)) * (R * (HD + 2)) + r; };
-    float acc[D] = {}, l = 0.f, m = -INFINITY;
+    float l = 0.f, m = -INFINITY;
+    if (few) {
+      float acc[DW] = {};
+#pragma unroll 2
+      for (int k = 0; k < n; ++k) {
+        const float* s = slot(k);
+        float x[DW];
+#pragma unroll
+        for (int i = 0; i < DW; ++i) x[i] = s[(team * DW + i) * R];
+        join(m, l, acc, s[HD * R], s[(HD + 1) * R], x);
+      }
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+      for (int i = 0; i < DW; i += 2) {
+        const float x = l == 0.f ? 0.f : acc[i] * inv, y = l == 0.f ? 0.f : acc[i + 1] * inv;
+        *reinterpret_cast<uint32_t*>(&out_s[lane][team * DW + i]) = p.is_bf16 ? pack2<true>(x, y) : pack2<false>(x, y);
+      }
+      if (team == 0 && r0 + lane < b.rows) store_lse(p, b.row0, b.row_lo + r, b.head, m, l);
+      __syncthreads();
+      for (int i = threadIdx.x; i < 32 * HD / 8; i += 256) {
+        const int row = i / (HD / 8), d = 8 * (i % (HD / 8)), of = b.row_lo + r0 + row, tok = of / p.group;
+        if (r0 + row >= b.rows) break;
+        uint16_t* const o = p.out + (int64_t)(b.row0 + tok) * p.out_stride + (int64_t)(b.head * p.group + of - tok * p.group) * HD + d;
+        if (p.vec_out16) {
+          *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(&out_s[row][d]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) o[e] = out_s[row][d + e];
+        }
+      }
+      __syncthreads();
+      return;
+    }
+    float acc[D] = {};
+#pragma unroll 2
     for (int k = team; k < n; k += 8) {
       const float* s = slot(k);
       float x[D];
 #pragma unroll
       for (int i = 0; i < D; ++i) x[i] = s[(d0 + i) * R];
-      const float mk = s[HD * R], lk = s[(HD + 1) * R], to = fmaxf(m, mk), base = to == -INFINITY ? 0.f : to;
-      const float f0 = ex2(m - base), f1 = ex2(mk - base);
-      m = to;
-      l = l * f0 + lk * f1;
-#pragma unroll
-      for (int i = 0; i < D; ++i) acc[i] = acc[i] * f0 + x[i] * f1;
+      join(m, l, acc, s[HD * R], s[(HD + 1) * R], x);
     }
 #pragma unroll
     for (int i = 0; i < D; ++i) acc_s[team][i][lane] = acc[i];
