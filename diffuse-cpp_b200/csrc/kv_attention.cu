@@ -694,7 +694,7 @@ template <int HD, int KV>
 struct TileCfg {
   static constexpr int R = 256, TILE = 128;
   static constexpr int ES = KV == KV_E4M3 ? 1 : 2;
-  static constexpr int OV = 2;
+  static constexpr int OV = 4;
   static constexpr int kThreads = 640, kLoaders = 128;
   // registers a thread: 256 * 160 + 256 * 64 + 128 * 32 = the 640 * 96 of the launch
   static constexpr int kSoftmaxRegs = 160, kLoadRegs = 64, kIssueRegs = 32;
@@ -1052,56 +1052,65 @@ __global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__
         }
       }
     };
+    // a thread turns its row into the products' type; f16 products: scaled into [-1, 1] by a power of two. The factor
+    // that turns the row's products into scores
+    auto ready_queries = [&]() {
+      float factor = p.scale_log2;
+      if (!w.more()) return factor;
+      if (half * 128 < w.it.rows) {
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        __syncwarp();
+        if (!(kBf && p.is_bf16)) {
+          uint8_t* const mine = q_warp + lane * 128;
+          auto piece = [&](int i) { return reinterpret_cast<uint4*>(mine + (i / 8) * C::kPlane + 16 * ((i % 8) ^ (lane & 7))); };
+          float inv = 1.f;
+          if (!kBf) {
+            uint32_t a = 0;  // magnitudes compare as integers
+#pragma unroll 4
+            for (int i = 0; i < HD / 8; ++i) {
+              const uint4 v = *piece(i);
+              a = __vmaxu2(a, __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
+            }
+            a = max(a & 0xffffu, a >> 16);
+            const float amax = p.is_bf16 ? __uint_as_float(a << 16) : __half2float(__ushort_as_half((uint16_t)a));
+            const int e = min(max((int)(__float_as_uint(amax) >> 23) - 126, -100), 100);
+            inv = pow2i(-e);
+            factor *= pow2i(e);
+          }
+#pragma unroll 2
+          for (int i = 0; i < HD / 8; ++i) {
+            const uint4 x = *piece(i);
+            uint32_t v[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float2 f = p.is_bf16 ? make_float2(__uint_as_float(v[k] << 16), __uint_as_float(v[k] & 0xffff0000u))
+                                         : __half22float2(*reinterpret_cast<const __half2*>(&v[k]));
+              v[k] = pack2<kBf>(f.x * inv, f.y * inv);
+            }
+            *piece(i) = make_uint4(v[0], v[1], v[2], v[3]);
+          }
+        }
+        fence_proxy_async_smem();
+      }
+      mbar_arrive(&bar.q_full);
+      return factor;
+    };
     fetch_queries();
+    float next_factor = ready_queries();
     uint32_t n = 0;  // tiles
     while (ok && w.more()) {
       const int seg = w.seg, rows = w.it.rows;
       const bool active = half * 128 < rows, live = my < rows, whole = w.whole();
+      const float factor = next_factor;
       if (!whole && w.t0 == 0) begun = w.begun();
       if (!active) {
-        mbar_arrive(&bar.q_full);
         mbar_arrive(&bar.read[seg & 3]);
         n += w.t1 - w.t0;
         w.next();
         fetch_queries();
+        next_factor = ready_queries();
         continue;
       }
-      // a thread turns its row into the products' type; f16 products: scaled into [-1, 1] by a power of two
-      float factor = p.scale_log2;
-      asm volatile("cp.async.wait_all;" ::: "memory");
-      __syncwarp();
-      if (!(kBf && p.is_bf16)) {
-        uint8_t* const mine = q_warp + lane * 128;
-        auto piece = [&](int i) { return reinterpret_cast<uint4*>(mine + (i / 8) * C::kPlane + 16 * ((i % 8) ^ (lane & 7))); };
-        float inv = 1.f;
-        if (!kBf) {
-          uint32_t a = 0;  // magnitudes compare as integers
-#pragma unroll 4
-          for (int i = 0; i < HD / 8; ++i) {
-            const uint4 v = *piece(i);
-            a = __vmaxu2(a, __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
-          }
-          a = max(a & 0xffffu, a >> 16);
-          const float amax = p.is_bf16 ? __uint_as_float(a << 16) : __half2float(__ushort_as_half((uint16_t)a));
-          const int e = min(max((int)(__float_as_uint(amax) >> 23) - 126, -100), 100);
-          inv = pow2i(-e);
-          factor *= pow2i(e);
-        }
-#pragma unroll 2
-        for (int i = 0; i < HD / 8; ++i) {
-          const uint4 x = *piece(i);
-          uint32_t v[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float2 f = p.is_bf16 ? make_float2(__uint_as_float(v[k] << 16), __uint_as_float(v[k] & 0xffff0000u))
-                                       : __half22float2(*reinterpret_cast<const __half2*>(&v[k]));
-            v[k] = pack2<kBf>(f.x * inv, f.y * inv);
-          }
-          *piece(i) = make_uint4(v[0], v[1], v[2], v[3]);
-        }
-      }
-      fence_proxy_async_smem();
-      mbar_arrive(&bar.q_full);
       const int row = w.it.row_lo + my;
       const int lim_all = row_limit(p, w.it.q, w.it.row_lo + rows - 1);
       const int lim = live ? row_limit(p, w.it.q, row) : lim_all;
@@ -1211,7 +1220,10 @@ __global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__
       const Item it = w.it;
       const int head = w.head;
       w.next();
-      fetch_queries();  // the scores' last arrival: the operand is free. On their way during the last product
+      // the scores' last arrival: the operand is free. The next item's scores are computed while this one's
+      // output is written
+      fetch_queries();
+      next_factor = ready_queries();
       ok = warp_wait(&bar.o_full[half], ph_o, err, kTimeout);
       if (!ok) break;
       ph_o ^= 1;
@@ -1222,6 +1234,15 @@ __global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__
       // columns at a time, so that either is written in whole sectors
       float* const part = p.part + (int64_t)(2 * blockIdx.x + (t0 == 0 ? 1 : 0)) * C::kPart + my;
       uint8_t* const stage = out_s + warp * C::kOutWarp;
+      uint16_t* out_row[4];  // lane's rows 8 i + lane / 4, at its eight columns
+      {
+        const int tok0 = it.row_lo / p.group, g0 = it.row_lo - tok0 * p.group;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = g0 + half * 128 + quarter * 32 + 8 * i + lane / 4, tok = (int)((r * (uint64_t)p.group_magic) >> 28);
+          out_row[i] = p.out + (int64_t)(it.q.row0 + tok0 + tok) * p.out_stride + (int64_t)(head * p.group + r - tok * p.group) * HD + 8 * (lane % 4);
+        }
+      }
 #pragma unroll 1
       for (int d0 = 0; d0 < HD; d0 += 32) {
         uint32_t x[32];
@@ -1258,8 +1279,7 @@ __global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__
           const int r = 8 * i + lane / 4, of = half * 128 + quarter * 32 + r;
           const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 64 + 16 * ((lane % 4) ^ ((r >> 1) & 3)));
           if (of < rows) {
-            const int orow = it.row_lo + of, tok = orow / p.group;
-            uint16_t* const o = p.out + (int64_t)(it.q.row0 + tok) * p.out_stride + (int64_t)(head * p.group + orow - tok * p.group) * HD + d0 + 8 * (lane % 4);
+            uint16_t* const o = out_row[i] + d0;
             if (p.vec_out16) {
               *reinterpret_cast<uint4*>(o) = v;
             } else {
