@@ -22,6 +22,7 @@
 
 #include "dmoe_internal.h"
 #include "kv_common.cuh"
+#include "sm100.cuh"
 
 namespace dmoe {
 
@@ -30,6 +31,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxHalf = 64;  // rotary_dim / 2 at head_dim 128
+constexpr int kWanted = 148 * 6;  // CTAs of a large call
 
 struct AppendParams {
   KvPages pg;
@@ -39,48 +41,57 @@ struct AppendParams {
   const float* q_norm;
   const float* k_norm;
   int64_t qkv_stride, q_stride;
-  int qkv_type, q_type;
+  int q_type;
   int n_head;
   int half;          // rotary_dim / 2
   int flat_slots;    // heads of the independent rows: [0, flat_slots)
-  int flat_per_cta, flat_groups, held_per_cta;
+  int flat_per_cta, flat_groups;  // heads a CTA takes of them, and how many such groups
+  int held_per_cta, held_groups;  // the same of the key heads, and of the value heads, of 8-bit pages
   int vec_in, vec_out;  // rows are 16-byte aligned
   float eps;
   double turns[kMaxHalf];  // base^(-2i / rotary_dim) / 2 pi
 };
 
-// 8 consecutive elements as floats. Every type is a vector of 16-byte loads when `vec`.
-__device__ __forceinline__ void load8(const void* p, int64_t at, int type, int vec, float (&x)[8]) {
-  if (type == DMOE_TYPE_F32) {
-    const float* f = static_cast<const float*>(p) + at;
+// 8 consecutive elements as they are, by 16-byte loads when `vec`, and as floats.
+template <int IN>
+struct Raw8 {
+  uint32_t w[IN == DMOE_TYPE_F32 ? 8 : 4];
+  __device__ __forceinline__ void load(const void* p, int64_t at, int vec) {
+    constexpr int N = IN == DMOE_TYPE_F32 ? 2 : 1;
     if (vec) {
-      const float4 a = __ldcs(reinterpret_cast<const float4*>(f)), b = __ldcs(reinterpret_cast<const float4*>(f) + 1);
-      x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+      const uint4* s = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p) + at * (IN == DMOE_TYPE_F32 ? 4 : 2));
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const uint4 v = __ldcs(s + i);
+        w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+      }
+    } else if (IN == DMOE_TYPE_F32) {
+#pragma unroll
+      for (int i = 0; i < 4 * N; ++i) w[i] = __ldcs(static_cast<const uint32_t*>(p) + at + i);
     } else {
+      const uint16_t* h = static_cast<const uint16_t*>(p) + at;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = __ldcs(f + i);
-    }
-    return;
-  }
-  uint32_t w[4];
-  const uint16_t* h = static_cast<const uint16_t*>(p) + at;
-  if (vec) {
-    const uint4 a = __ldcs(reinterpret_cast<const uint4*>(h));
-    w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = __ldcs(h + 2 * i) | ((uint32_t)__ldcs(h + 2 * i + 1) << 16);
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (type == DMOE_TYPE_F16) {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-      x[2 * i] = f.x, x[2 * i + 1] = f.y;
-    } else {
-      x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      for (int i = 0; i < 4; ++i) w[i] = __ldcs(h + 2 * i) | ((uint32_t)__ldcs(h + 2 * i + 1) << 16);
     }
   }
-}
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < (IN == DMOE_TYPE_F32 ? 8 : 4); ++i) w[i] = 0;
+  }
+  __device__ __forceinline__ void get(float (&x)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (IN == DMOE_TYPE_F32) {
+        x[2 * i] = __uint_as_float(w[2 * i]), x[2 * i + 1] = __uint_as_float(w[2 * i + 1]);
+      } else if constexpr (IN == DMOE_TYPE_F16) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        x[2 * i] = f.x, x[2 * i + 1] = f.y;
+      } else {
+        x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      }
+    }
+  }
+};
 
 __device__ __forceinline__ uint4 pack8(const float (&x)[8], int type) {
   uint32_t w[4];
@@ -186,7 +197,7 @@ __device__ __forceinline__ void dequantise8(uint2 w, float scale, float (&x)[8])
     }
 }
 
-template <int HD, int KV>
+template <int HD, int KV, int IN>
 __global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_constant__ AppendParams p) {
   constexpr int LPR = HD / 8;     // lanes a row
   constexpr int RPW = 32 / LPR;   // rows a warp holds at once
@@ -195,6 +206,7 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_consta
   __shared__ float amax_s[2][kWarps];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, sub = lane % LPR;
 
+  pdl_wait();
   // this CTA's unit: block `rel` among those of sequence `s` that gain rows
   int s = -1, rel = (int)blockIdx.x;
   KvSeq q{};
@@ -241,8 +253,9 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_consta
   const int64_t row_lo = (int64_t)q.row0 + (lo - pos0);  // row of position lo
   const int group = (int)blockIdx.y;
 
-  // (cos, sin) of the block's new positions, once for all heads of the CTA
-  for (int i = tid; i < fresh * p.half; i += kThreads) {
+  // (cos, sin) of the block's new positions, once for all heads of the CTA; values are not rotated
+  const bool values = group >= p.flat_groups + p.held_groups;
+  for (int i = tid; i < (values ? 0 : fresh * p.half); i += kThreads) {
     const int t = i / p.half, f = i % p.half;
     const double a = (double)(lo + t) * p.turns[f];
     float sn, c;
@@ -263,25 +276,31 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_consta
                  p.vec_out, zero);
       }
     }
-    for (int r0 = warp * RPW; r0 < fresh * nh; r0 += kWarps * RPW) {
-      const int r = r0 + lane / LPR;
-      const bool live = r < fresh * nh;
-      const int t = live ? r % fresh : 0, h = h0 + (live ? r / fresh : 0);
-      float x[8] = {};
-      if (live) load8(p.qkv, (row_lo + t) * p.qkv_stride + (int64_t)h * HD + 8 * sub, p.qkv_type, p.vec_in, x);
-      const float2* c = cs + (lo - b0 + t) * kMaxHalf;
-      if (KV == KV_E4M3) {
-        norm_rotate<LPR>(x, p.q_norm, p.q_norm != nullptr, p.eps, sub, p.half, c);
-        if (live) store8(p.q_out, (row_lo + t) * p.q_stride + (int64_t)h * HD + 8 * sub, p.q_type, p.vec_out, x);
-      } else {
+    // four rows a lane on their way at once
+    constexpr int U = IN == DMOE_TYPE_F32 ? 2 : 4;
+    for (int r0 = warp * RPW; r0 < fresh * nh; r0 += kWarps * RPW * U) {
+      Raw8<IN> raw[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int r = r0 + u * kWarps * RPW + lane / LPR;
+        raw[u].zero();
+        if (r < fresh * nh) raw[u].load(p.qkv, (row_lo + r % fresh) * p.qkv_stride + (int64_t)(h0 + r / fresh) * HD + 8 * sub, p.vec_in);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int r = r0 + u * kWarps * RPW + lane / LPR;
+        if (r0 + u * kWarps * RPW >= fresh * nh) break;  // the whole warp
+        const bool live = r < fresh * nh;
+        const int t = live ? r % fresh : 0, h = h0 + (live ? r / fresh : 0);
         const bool is_q = h < p.n_head, is_v = h >= p.n_head + p.pg.n_head_kv;
-        float y[8];
+        float x[8], y[8];
+        raw[u].get(x);
 #pragma unroll
         for (int i = 0; i < 8; ++i) y[i] = x[i];
-        const float* w = is_q ? p.q_norm : p.k_norm;
-        norm_rotate<LPR>(y, w, w != nullptr && !is_v, p.eps, sub, p.half, c);
+        const float* w = KV == KV_E4M3 || is_q ? p.q_norm : p.k_norm;
+        norm_rotate<LPR>(y, w, w != nullptr && (KV == KV_E4M3 || !is_v), p.eps, sub, p.half, cs + (lo - b0 + t) * kMaxHalf);
         if (!live) continue;
-        if (is_q) {
+        if (KV == KV_E4M3 || is_q) {
           store8(p.q_out, (row_lo + t) * p.q_stride + (int64_t)h * HD + 8 * sub, p.q_type, p.vec_out, y);
         } else if (page >= 0) {
           const int hk = is_v ? h - p.n_head - p.pg.n_head_kv : h - p.n_head;
@@ -296,27 +315,32 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_consta
   }
   if (KV != KV_E4M3 || fresh == 0 || page < 0) return;
 
-  const int hs0 = (group - p.flat_groups) * p.held_per_cta, hs1 = min(hs0 + p.held_per_cta, 2 * p.pg.n_head_kv);
-  for (int hs = hs0; hs < hs1; ++hs) {
-    const bool is_v = hs >= p.pg.n_head_kv;
-    const int hk = is_v ? hs - p.pg.n_head_kv : hs;
+  const bool is_v = values;
+  const int hk0 = (group - p.flat_groups - (values ? p.held_groups : 0)) * p.held_per_cta, hk1 = min(hk0 + p.held_per_cta, p.pg.n_head_kv);
+  for (int hk = hk0; hk < hk1; ++hk) {
+    const int hs = (is_v ? p.pg.n_head_kv : 0) + hk;
     uint8_t* codes = static_cast<uint8_t*>(is_v ? p.pg.v : p.pg.k);
     uint8_t* sc = (is_v ? p.pg.v_scale : p.pg.k_scale) +
                   ((page * p.pg.n_head_kv + hk) * p.pg.page_size + off0) / kScaleBlock;
     const int e_old = lo > b0 ? (int)*sc - 127 : kExpMin;
     float x[PASSES][8];
     float amax = 0.f;
+    {
+      Raw8<IN> raw[PASSES];
+      uint2 kept[PASSES];
 #pragma unroll
-    for (int j = 0; j < PASSES; ++j) {
-      const int t = (j * kWarps + warp) * RPW + lane / LPR, pos = b0 + t;
+      for (int j = 0; j < PASSES; ++j) {
+        const int t = (j * kWarps + warp) * RPW + lane / LPR, pos = b0 + t;
+        raw[j].zero();
+        if (pos >= lo && pos < hi)
+          raw[j].load(p.qkv, (row_lo + (pos - lo)) * p.qkv_stride + (int64_t)(p.n_head + hs) * HD + 8 * sub, p.vec_in);
+        else if (pos < lo)
+          kept[j] = *reinterpret_cast<const uint2*>(codes + kv_row(p.pg, page, hk, off0 + t) * HD + 8 * sub);
+      }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[j][i] = 0.f;
-      if (pos >= lo && pos < hi) {
-        load8(p.qkv, (row_lo + (pos - lo)) * p.qkv_stride + (int64_t)(p.n_head + hs) * HD + 8 * sub, p.qkv_type,
-              p.vec_in, x[j]);
-      } else if (pos < lo) {
-        const uint2 w = *reinterpret_cast<const uint2*>(codes + kv_row(p.pg, page, hk, off0 + t) * HD + 8 * sub);
-        dequantise8(w, exp2f((float)e_old), x[j]);
+      for (int j = 0; j < PASSES; ++j) {
+        raw[j].get(x[j]);
+        if (b0 + (j * kWarps + warp) * RPW + lane / LPR < lo) dequantise8(kept[j], exp2f((float)e_old), x[j]);
       }
     }
 #pragma unroll
@@ -339,10 +363,10 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_consta
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    if (lane == 0) amax_s[hs & 1][warp] = amax;
+    if (lane == 0) amax_s[hk & 1][warp] = amax;
     __syncthreads();  // also: every thread has read the old scale
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) amax = fmaxf(amax, amax_s[hs & 1][w]);
+    for (int w = 0; w < kWarps; ++w) amax = fmaxf(amax, amax_s[hk & 1][w]);
     const int e = scale_exponent(amax);
     const float inv = exp2f((float)-e);
 #pragma unroll
@@ -353,6 +377,16 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_consta
     }
     if (tid == 0) *sc = (uint8_t)(e + 127);
   }
+}
+
+template <int IN>
+cudaError_t launch_append(const AppendParams& p, int hd, KvType kv, dim3 grid, cudaStream_t st) {
+  void (*k)(AppendParams);
+  if (hd == 128)
+    k = kv == KV_BF16 ? kv_append_kernel<128, KV_BF16, IN> : kv == KV_F16 ? kv_append_kernel<128, KV_F16, IN> : kv_append_kernel<128, KV_E4M3, IN>;
+  else
+    k = kv == KV_BF16 ? kv_append_kernel<64, KV_BF16, IN> : kv == KV_F16 ? kv_append_kernel<64, KV_F16, IN> : kv_append_kernel<64, KV_E4M3, IN>;
+  return launch_pdl(k, grid, dim3(kThreads), 0, st, p);
 }
 
 bool is_float_type(int t) { return t == DMOE_TYPE_F32 || t == DMOE_TYPE_F16 || t == DMOE_TYPE_BF16; }
@@ -435,7 +469,6 @@ extern "C" dmoe_status dmoe_kv_append(const dmoe_kv_cache* cache, const dmoe_kv_
   p.k_norm = a->k_norm;
   p.qkv_stride = a->qkv_stride;
   p.q_stride = a->q_stride;
-  p.qkv_type = a->qkv_type;
   p.q_type = a->q_type;
   p.n_head = a->n_head;
   p.half = a->rotary_dim / 2;
@@ -451,21 +484,30 @@ extern "C" dmoe_status dmoe_kv_append(const dmoe_kv_cache* cache, const dmoe_kv_
   const KvType kv = kv_type_of(cache->type);
   // a sequence of f new rows touches at most f blocks, and at most f / 32 + 2
   const int64_t units = std::min<int64_t>(a->n_tokens, a->n_tokens / kScaleBlock + 2ll * batch->n_seq);
-  const int held = kv == KV_E4M3 ? 2 * nk : 0;
-  p.flat_slots = a->n_head + 2 * nk - held;
-  p.flat_per_cta = p.flat_slots;
-  p.held_per_cta = std::max(1, held);
-  p.flat_groups = 1;
-  const int groups = p.flat_groups + (held ? 1 : 0);
-  const dim3 grid((unsigned)units, (unsigned)groups);
+  const bool held = kv == KV_E4M3;
+  p.flat_slots = a->n_head + (held ? 0 : 2 * nk);
+  // Heads a CTA takes: as many as leave about kWanted CTAs (the rotation's table is then made for several heads; one
+  // head each below that, where latency counts), but at least the 16 rows that the warps hold at once
+  const int64_t fresh = std::max<int64_t>(1, std::min<int64_t>(kScaleBlock, a->n_tokens / std::max<int64_t>(1, units)));
+  auto share = [&](int64_t heads, int64_t least) {
+    const int64_t per = std::max((units * heads + kWanted - 1) / kWanted, least), groups = (heads + per - 1) / per;
+    return (int)((heads + groups - 1) / groups);  // even groups
+  };
+  p.flat_per_cta = share(p.flat_slots, std::min<int64_t>(p.flat_slots, (16 + fresh - 1) / fresh));
+  p.flat_groups = (p.flat_slots + p.flat_per_cta - 1) / p.flat_per_cta;
+  p.held_per_cta = held ? share(nk, 1) : 1;
+  p.held_groups = held ? (nk + p.held_per_cta - 1) / p.held_per_cta : 0;
+  const dim3 grid((unsigned)units, (unsigned)(p.flat_groups + 2 * p.held_groups));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  void (*kernel)(AppendParams) = nullptr;
-  if (hd == 128)
-    kernel = kv == KV_BF16 ? kv_append_kernel<128, KV_BF16> : kv == KV_F16 ? kv_append_kernel<128, KV_F16> : kv_append_kernel<128, KV_E4M3>;
+  set_pdl_for_call(true);
+  cudaError_t e;
+  if (a->qkv_type == DMOE_TYPE_F32)
+    e = launch_append<DMOE_TYPE_F32>(p, hd, kv, grid, st);
+  else if (a->qkv_type == DMOE_TYPE_F16)
+    e = launch_append<DMOE_TYPE_F16>(p, hd, kv, grid, st);
   else
-    kernel = kv == KV_BF16 ? kv_append_kernel<64, KV_BF16> : kv == KV_F16 ? kv_append_kernel<64, KV_F16> : kv_append_kernel<64, KV_E4M3>;
-  kernel<<<grid, kThreads, 0, st>>>(p);
-  const cudaError_t e = cudaGetLastError();
+    e = launch_append<DMOE_TYPE_BF16>(p, hd, kv, grid, st);
+  set_pdl_for_call(false);
   if (e != cudaSuccess) {
     char msg[256];
     snprintf(msg, sizeof(msg), "launch failed: %s", cudaGetErrorString(e));
