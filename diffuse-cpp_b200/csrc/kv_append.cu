@@ -131,32 +131,42 @@ __device__ __forceinline__ void store8(void* p, int64_t at, int type, int vec, c
   }
 }
 
+// A lane's 8 weights of a norm; ones where there is none.
+__device__ __forceinline__ void load_weights(const float* w, int sub, float (&g)[8]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float4 v = w ? __ldg(reinterpret_cast<const float4*>(w) + 2 * sub + i) : make_float4(1.f, 1.f, 1.f, 1.f);
+    g[4 * i] = v.x, g[4 * i + 1] = v.y, g[4 * i + 2] = v.z, g[4 * i + 3] = v.w;
+  }
+}
+
 // y = norm(x) * w, then the rotation; every lane of the warp takes part (LPR lanes hold one row).
 // cs: the row's (cos, sin) pairs.
 template <int LPR>
-__device__ __forceinline__ void norm_rotate(float (&x)[8], const float* __restrict__ w, bool norm, float eps, int sub,
-                                            int half, const float2* cs) {
+__device__ __forceinline__ void norm_rotate(float (&x)[8], const float (&w)[8], bool norm, float eps, int sub, int half,
+                                            const float2* cs) {
   float ss = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
 #pragma unroll
   for (int o = LPR / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  if (norm) {
-    const float r = 1.0f / sqrtf(ss * (1.0f / (8 * LPR)) + eps);
-    const float4 a = __ldg(reinterpret_cast<const float4*>(w) + 2 * sub), b = __ldg(reinterpret_cast<const float4*>(w) + 2 * sub + 1);
-    x[0] *= r * a.x, x[1] *= r * a.y, x[2] *= r * a.z, x[3] *= r * a.w;
-    x[4] *= r * b.x, x[5] *= r * b.y, x[6] *= r * b.z, x[7] *= r * b.w;
-  }
+  const float r = norm ? 1.0f / sqrtf(ss * (1.0f / (8 * LPR)) + eps) : 1.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] *= r * w[i];
   if (half == 0) return;
   const int hl = half / 8;
   const bool lo = sub < hl, in = sub < 2 * hl;
   const int lane = threadIdx.x & 31, from = lane + (lo ? hl : in ? -hl : 0);
-  const float2* c = cs + 8 * (lo ? sub : in ? sub - hl : 0);
+  const float4* c = reinterpret_cast<const float4*>(cs + 8 * (lo ? sub : in ? sub - hl : 0));
+  const float sign = lo ? -1.f : 1.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float y = __shfl_sync(0xffffffffu, x[i], from);
-    const float2 t = c[i];
-    if (in) x[i] = lo ? x[i] * t.x - y * t.y : x[i] * t.x + y * t.y;
+  for (int i = 0; i < 8; i += 2) {
+    const float y0 = __shfl_sync(0xffffffffu, x[i], from), y1 = __shfl_sync(0xffffffffu, x[i + 1], from);
+    const float4 t = c[i / 2];
+    if (in) {
+      x[i] = fmaf(x[i], t.x, sign * (y0 * t.y));
+      x[i + 1] = fmaf(x[i + 1], t.z, sign * (y1 * t.w));
+    }
   }
 }
 
@@ -202,7 +212,7 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_consta
   constexpr int LPR = HD / 8;     // lanes a row
   constexpr int RPW = 32 / LPR;   // rows a warp holds at once
   constexpr int PASSES = kScaleBlock / (kWarps * RPW);
-  __shared__ float2 cs[kScaleBlock * kMaxHalf];
+  __shared__ __align__(16) float2 cs[kScaleBlock * kMaxHalf];
   __shared__ float amax_s[2][kWarps];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, sub = lane % LPR;
 
@@ -276,6 +286,11 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_consta
                  p.vec_out, zero);
       }
     }
+    float wq[8], wk[8];
+    load_weights(p.q_norm, sub, wq);
+    load_weights(KV == KV_E4M3 ? p.q_norm : p.k_norm, sub, wk);
+    // r / fresh for r < 2^13 (at most 128 heads a CTA) and fresh <= 32: r * (magic * fresh - 2^18) < 2^18
+    const uint32_t magic = fresh ? ((1u << 18) + fresh - 1) / fresh : 0;
     // four rows a lane on their way at once
     constexpr int U = IN == DMOE_TYPE_F32 ? 2 : 4;
     for (int r0 = warp * RPW; r0 < fresh * nh; r0 += kWarps * RPW * U) {
@@ -284,21 +299,31 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_consta
       for (int u = 0; u < U; ++u) {
         const int r = r0 + u * kWarps * RPW + lane / LPR;
         raw[u].zero();
-        if (r < fresh * nh) raw[u].load(p.qkv, (row_lo + r % fresh) * p.qkv_stride + (int64_t)(h0 + r / fresh) * HD + 8 * sub, p.vec_in);
+        if (r < fresh * nh) {
+          const int h = (int)((r * magic) >> 18);
+          raw[u].load(p.qkv, (row_lo + r - h * fresh) * p.qkv_stride + (int64_t)(h0 + h) * HD + 8 * sub, p.vec_in);
+        }
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int r = r0 + u * kWarps * RPW + lane / LPR;
         if (r0 + u * kWarps * RPW >= fresh * nh) break;  // the whole warp
         const bool live = r < fresh * nh;
-        const int t = live ? r % fresh : 0, h = h0 + (live ? r / fresh : 0);
+        const int hr = live ? (int)((r * magic) >> 18) : 0, t = live ? r - hr * fresh : 0, h = h0 + hr;
         const bool is_q = h < p.n_head, is_v = h >= p.n_head + p.pg.n_head_kv;
         float x[8], y[8];
         raw[u].get(x);
 #pragma unroll
         for (int i = 0; i < 8; ++i) y[i] = x[i];
-        const float* w = KV == KV_E4M3 || is_q ? p.q_norm : p.k_norm;
-        norm_rotate<LPR>(y, w, w != nullptr && (KV == KV_E4M3 || !is_v), p.eps, sub, p.half, cs + (lo - b0 + t) * kMaxHalf);
+        const float2* const c = cs + (lo - b0 + t) * kMaxHalf;
+        if (KV == KV_E4M3) {
+          norm_rotate<LPR>(y, wq, p.q_norm != nullptr, p.eps, sub, p.half, c);
+        } else {
+          float w[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) w[i] = is_q ? wq[i] : wk[i];
+          norm_rotate<LPR>(y, w, (is_q ? p.q_norm : p.k_norm) != nullptr, p.eps, sub, p.half, c);
+        }
         if (!live) continue;
         if (KV == KV_E4M3 || is_q) {
           store8(p.q_out, (row_lo + t) * p.q_stride + (int64_t)h * HD + 8 * sub, p.q_type, p.vec_out, y);
@@ -316,6 +341,8 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_consta
   if (KV != KV_E4M3 || fresh == 0 || page < 0) return;
 
   const bool is_v = values;
+  float wk[8];
+  load_weights(is_v ? nullptr : p.k_norm, sub, wk);
   const int hk0 = (group - p.flat_groups - (values ? p.held_groups : 0)) * p.held_per_cta, hk1 = min(hk0 + p.held_per_cta, p.pg.n_head_kv);
   for (int hk = hk0; hk < hk1; ++hk) {
     const int hs = (is_v ? p.pg.n_head_kv : 0) + hk;
@@ -351,7 +378,7 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_consta
 #pragma unroll
         for (int i = 0; i < 8; ++i) y[i] = x[j][i];
         const bool now = b0 + t >= lo && b0 + t < hi;
-        norm_rotate<LPR>(y, p.k_norm, p.k_norm != nullptr, p.eps, sub, p.half, cs + (now ? t : lo - b0) * kMaxHalf);
+        norm_rotate<LPR>(y, wk, p.k_norm != nullptr, p.eps, sub, p.half, cs + (now ? t : lo - b0) * kMaxHalf);
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[j][i] = now ? y[i] : x[j][i];
       }
@@ -490,7 +517,7 @@ extern "C" dmoe_status dmoe_kv_append(const dmoe_kv_cache* cache, const dmoe_kv_
   // head each below that, where latency counts), but at least the 16 rows that the warps hold at once
   const int64_t fresh = std::max<int64_t>(1, std::min<int64_t>(kScaleBlock, a->n_tokens / std::max<int64_t>(1, units)));
   auto share = [&](int64_t heads, int64_t least) {
-    const int64_t per = std::max((units * heads + kWanted - 1) / kWanted, least), groups = (heads + per - 1) / per;
+    const int64_t per = std::min<int64_t>(128, std::max((units * heads + kWanted - 1) / kWanted, least)), groups = (heads + per - 1) / per;
     return (int)((heads + groups - 1) / groups);  // even groups
   };
   p.flat_per_cta = share(p.flat_slots, std::min<int64_t>(p.flat_slots, (16 + fresh - 1) / fresh));
