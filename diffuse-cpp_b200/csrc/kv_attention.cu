@@ -19,6 +19,7 @@
 // ones share a CTA. An item that spans CTAs leaves partial (o, M, sum) triples in the workspace, which
 // kv_combine_kernel adds in a fixed order (results do not depend on timing).
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdio>
 
@@ -1492,33 +1493,38 @@ constexpr int kTileGrid = kMaxGrid;
 constexpr int kCombineGrid = 8 * kMaxGrid;
 constexpr int kRowsMax = 16;  // rows of a sequence and key/value head that the few-rows kernel takes
 
+// The shared memory limit of a kernel, raised once on each device.
+template <typename F>
+cudaError_t allow_smem(F kernel, size_t bytes, std::atomic<uint64_t>& seen) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (dev < 64 && (seen.load(std::memory_order_relaxed) >> dev & 1))) return e;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e == cudaSuccess && dev < 64) seen.fetch_or(uint64_t{1} << dev, std::memory_order_relaxed);
+  return e;
+}
+
 template <int HD, int KV, int NT>
 cudaError_t launch_rows(AttnParams p, int max_rows, cudaStream_t st) {
   using C = RowsCfg<HD, KV, NT>;
+  static std::atomic<uint64_t> seen{0};
   p.n_qt = (max_rows + C::R - 1) / C::R;
   static_assert(C::kSmem <= 227 * 1024, "shared memory");
-  cudaError_t e = cudaFuncSetAttribute(kv_rows_kernel<HD, KV, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmem);
-  if (e != cudaSuccess) return e;
-  set_pdl_for_call(true);
-  e = launch_pdl(kv_rows_kernel<HD, KV, NT>, dim3(kRowsGrid), dim3(256), C::kSmem, st, p);
-  if (e != cudaSuccess) return e;
-  e = launch_pdl(kv_combine_kernel<HD, C::R>, dim3(kCombineGrid), dim3(256), 0, st, p, kRowsGrid);
-  set_pdl_for_call(false);
+  cudaError_t e = allow_smem(kv_rows_kernel<HD, KV, NT>, C::kSmem, seen);
+  if (e == cudaSuccess) e = launch_pdl(kv_rows_kernel<HD, KV, NT>, dim3(kRowsGrid), dim3(256), C::kSmem, st, p);
+  if (e == cudaSuccess) e = launch_pdl(kv_combine_kernel<HD, C::R>, dim3(kCombineGrid), dim3(256), 0, st, p, kRowsGrid);
   return e;
 }
 
 template <int HD, int KV>
 cudaError_t launch_tiles(AttnParams p, int max_rows, cudaStream_t st) {
   using C = TileCfg<HD, KV>;
+  static std::atomic<uint64_t> seen{0};
   p.n_qt = (max_rows + C::R - 1) / C::R;
   static_assert(C::kSmem <= 220 * 1024, "shared memory");
-  cudaError_t e = cudaFuncSetAttribute(kv_tile_kernel<HD, KV>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmem);
-  if (e != cudaSuccess) return e;
-  set_pdl_for_call(true);
-  e = launch_pdl(kv_tile_kernel<HD, KV>, dim3(kTileGrid), dim3(C::kThreads), C::kSmem, st, p);
-  if (e != cudaSuccess) return e;
-  e = launch_pdl(kv_combine_tiles_kernel<HD, C::R>, dim3(kCombineGrid), dim3(256), 0, st, p, kTileGrid);
-  set_pdl_for_call(false);
+  cudaError_t e = allow_smem(kv_tile_kernel<HD, KV>, C::kSmem, seen);
+  if (e == cudaSuccess) e = launch_pdl(kv_tile_kernel<HD, KV>, dim3(kTileGrid), dim3(C::kThreads), C::kSmem, st, p);
+  if (e == cudaSuccess) e = launch_pdl(kv_combine_tiles_kernel<HD, C::R>, dim3(kCombineGrid), dim3(256), 0, st, p, kTileGrid);
   return e;
 }
 
@@ -1612,10 +1618,12 @@ extern "C" dmoe_status dmoe_kv_attention(const dmoe_kv_cache* cache, const dmoe_
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const KvType kv = kv_type_of(cache->type);
   cudaError_t e;
+  set_pdl_for_call(true);
   if (hd == 128)
     e = kv == KV_BF16 ? launch_kv<128, KV_BF16>(p, max_rows, st) : kv == KV_F16 ? launch_kv<128, KV_F16>(p, max_rows, st) : launch_kv<128, KV_E4M3>(p, max_rows, st);
   else
     e = kv == KV_BF16 ? launch_kv<64, KV_BF16>(p, max_rows, st) : kv == KV_F16 ? launch_kv<64, KV_F16>(p, max_rows, st) : launch_kv<64, KV_E4M3>(p, max_rows, st);
+  set_pdl_for_call(false);
   if (e != cudaSuccess) {
     char msg[256];
     snprintf(msg, sizeof(msg), "launch failed: %s", cudaGetErrorString(e));

@@ -12,9 +12,9 @@ stream and `sync()` waits for it).
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import os
+import struct
 from typing import Optional
 
 import numpy as np
@@ -187,6 +187,12 @@ class KVAttentionArgs(ctypes.Structure):
         ("block_length", ctypes.c_int32),
         ("scale", ctypes.c_float),
     ]
+
+
+# the same two as bytes (native alignment): packed in one step, the cost of a call counts
+_APPEND_ARGS = struct.Struct("@PPPPqqqiiiifd")
+_ATTENTION_ARGS = struct.Struct("@PPPqqqiiif")
+assert _APPEND_ARGS.size == ctypes.sizeof(KVAppendArgs) and _ATTENTION_ARGS.size == ctypes.sizeof(KVAttentionArgs)
 
 
 class DmoeError(RuntimeError):
@@ -603,31 +609,33 @@ class PagedKV:
             self._desc.append(KVCacheDesc(_ptr(self.k[il]), _ptr(self.v[il]), *sc, _ptr(self.err), n_pages, n_head_kv,
                                           head_dim, page_size, ctype))
         self._ref = [ctypes.addressof(d) for d in self._desc]
+        self._lib, self._f32, self._norm_shape, self._scale = load(), torch.float32, (head_dim,), head_dim ** -0.5
 
     def _rows(self, call: str, name: str, t, width: int, n: int = -1):
         """Checks a row tensor ([n, width] elements, rows any distance apart); its type id and row stride."""
-        kind = self._types.get(t.dtype)
+        kind, shape, stride = self._types.get(t.dtype), t.shape, t.stride()
         if kind is None or t.device != self.device:
             raise ValueError(f"{call}: {name} must be a float32, float16 or bfloat16 tensor on {self.device}")
-        shape = t.shape
-        dense = len(shape) == 2 and shape[1] == width and (t.stride(1) == 1 or width == 1)
-        if not dense and len(shape) == 3:
-            dense = shape[1] * shape[2] == width and t.stride(2) == 1 and t.stride(1) == shape[2]
+        if len(shape) == 3:
+            dense = shape[1] * shape[2] == width and stride[2] == 1 and stride[1] == shape[2]
+        else:
+            dense = len(shape) == 2 and shape[1] == width and (stride[1] == 1 or width == 1)
         if not dense or (n >= 0 and shape[0] != n):
             raise ValueError(f"{call}: {name} must hold {'n' if n < 0 else n} rows of {width} consecutive elements")
-        return kind, t.stride(0) if shape[0] > 1 else max(width, t.stride(0))
+        return kind, stride[0] if shape[0] > 1 else max(width, stride[0])
 
-    def _launch(self, batch: KVBatch, stream, fn):
+    def _launch(self, batch: KVBatch, stream, fn, *args):
+        """fn(stream, *args) with the cache's device current; `stream` None: the current torch stream."""
         import torch
 
         if batch.device != self.device:
             raise ValueError("PagedKV: the batch and the cache are on different devices")
         if stream is None:
-            stream = torch.cuda.current_stream(self.device).cuda_stream
-        if torch.cuda.current_device() != self.device.index:
+            stream = torch._C._cuda_getCurrentRawStream(self.device.index)
+        if torch._C._cuda_getDevice() != self.device.index:
             with torch.cuda.device(self.device):
-                return fn(stream)
-        return fn(stream)
+                return fn(stream or None, *args)
+        return fn(stream or None, *args)
 
     def append(self, layer: int, qkv, batch: KVBatch, n_head: int, q_norm=None, k_norm=None, eps: float = 1e-6,
                rotary_dim: int = 0, rope_base: float = 10000.0, q_type=None, q_out=None, stream: Optional[int] = None):
@@ -635,22 +643,22 @@ class PagedKV:
         queries [n, n_head, head_dim] (q_out, or a new tensor of q_type, default qkv's). q_norm and k_norm:
         [head_dim] float32, or None for no normalisation. Rows that belong to no sequence are not
         written: in a new tensor they are uninitialised."""
-        import torch
-
-        n = int(qkv.shape[0])
         kind, stride = self._rows("append", "qkv", qkv, (n_head + 2 * self.n_head_kv) * self.head_dim)
+        n = qkv.shape[0]
         if q_out is None:
-            q_out = torch.empty((n, n_head, self.head_dim), dtype=q_type or qkv.dtype, device=self.device)
+            q_out = qkv.new_empty((n, n_head, self.head_dim), dtype=q_type)
         q_kind, q_stride = self._rows("append", "q_out", q_out, n_head * self.head_dim, n)
         for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
-            if w is not None and (w.dtype != torch.float32 or w.device != self.device or w.shape != (self.head_dim,)
+            if w is not None and (w.shape != self._norm_shape or w.dtype != self._f32 or w.device != self.device
                                   or not w.is_contiguous()):
                 raise ValueError(f"append: {name} must be a contiguous float32 [head_dim] tensor on {self.device}")
-        args = KVAppendArgs(qkv.data_ptr(), q_out.data_ptr(), _ptr(q_norm) or None, _ptr(k_norm) or None, n, stride,
-                            q_stride, kind, q_kind, n_head, rotary_dim, eps, rope_base)
-        _check(self._launch(batch, stream, lambda st: load().dmoe_kv_append(
-            self._ref[layer], batch._ref, ctypes.addressof(args), st or None)))
+        args = _APPEND_ARGS.pack(qkv.data_ptr(), q_out.data_ptr(), _ptr(q_norm), _ptr(k_norm), n, stride, q_stride, kind,
+                                 q_kind, n_head, rotary_dim, eps, rope_base)
+        _check(self._launch(batch, stream, self._append, layer, batch, args))
         return q_out
+
+    def _append(self, stream, layer, batch, args):
+        return self._lib.dmoe_kv_append(self._ref[layer], batch._ref, args, stream)
 
     def attend(self, layer: int, q, batch: KVBatch, block_length: int = 1, scale: Optional[float] = None, out=None,
                lse=None, stream: Optional[int] = None):
@@ -658,35 +666,37 @@ class PagedKV:
         and type. A row at position p sees the positions j < kv_len with j // block_length <= p // block_length.
         scale: default head_dim ** -0.5. lse: [n, n_head] float32 for the logarithms of the softmax sums, or
         None. Rows that belong to no sequence are not written."""
-        import torch
-
-        if q.dim() != 3 or q.shape[2] != self.head_dim:
+        if len(q.shape) != 3 or q.shape[2] != self.head_dim:
             raise ValueError("attend: q must be [n, n_head, head_dim]")
-        n, n_head = int(q.shape[0]), int(q.shape[1])
+        n, n_head, _ = q.shape
         kind, stride = self._rows("attend", "q", q, n_head * self.head_dim)
         if out is None:
-            out = torch.empty((n, n_head, self.head_dim), dtype=q.dtype, device=self.device)
+            out = q.new_empty(q.shape)
         o_kind, o_stride = self._rows("attend", "out", out, n_head * self.head_dim, n)
         if o_kind != kind:
             raise ValueError("attend: out must have q's type")
-        if lse is not None and (lse.dtype != torch.float32 or lse.device != self.device or lse.shape != (n, n_head)
+        if lse is not None and (lse.dtype != self._f32 or lse.device != self.device or lse.shape != (n, n_head)
                                 or not lse.is_contiguous()):
             raise ValueError(f"attend: lse must be a contiguous float32 [n, n_head] tensor on {self.device}")
-        args = KVAttentionArgs(q.data_ptr(), out.data_ptr(), _ptr(lse) or None, n, stride, o_stride, kind, n_head,
-                               block_length, scale if scale is not None else self.head_dim ** -0.5)
-        lib, ref = load(), ctypes.addressof(args)
-
-        def call(st):
-            size = lib.dmoe_kv_attention_workspace(self._ref[layer], batch._ref, ref)
-            ws = None
-            if size:  # of the launching stream's pool: calls on different streams and graphs have their own
-                with torch.cuda.stream(torch.cuda.ExternalStream(st, device=self.device)) if stream is not None \
-                        else contextlib.nullcontext():
-                    ws = torch.empty(size, dtype=torch.uint8, device=self.device)
-            return lib.dmoe_kv_attention(self._ref[layer], batch._ref, ref, _ptr(ws) or None, size, st or None)
-
-        _check(self._launch(batch, stream, call))
+        args = _ATTENTION_ARGS.pack(q.data_ptr(), out.data_ptr(), _ptr(lse), n, stride, o_stride, kind, n_head,
+                                    block_length, scale if scale is not None else self._scale)
+        _check(self._launch(batch, stream, self._attend, layer, batch, args, stream))
         return out
+
+    def _attend(self, stream, layer, batch, args, given):
+        cache = self._ref[layer]
+        size = self._lib.dmoe_kv_attention_workspace(cache, batch._ref, args)
+        if not size:
+            return self._lib.dmoe_kv_attention(cache, batch._ref, args, None, 0, stream)
+        # of the launching stream's pool: calls on different streams and in different graphs have their own
+        if given is None:
+            ws = self.err.new_empty(size // 4)
+        else:
+            import torch
+
+            with torch.cuda.stream(torch.cuda.ExternalStream(given, device=self.device)):
+                ws = self.err.new_empty(size // 4)
+        return self._lib.dmoe_kv_attention(cache, batch._ref, args, ws.data_ptr(), size, stream)
 
     def check(self) -> None:
         """Waits for the device and raises if a kernel met a page number or a batch entry out of its bounds
