@@ -611,6 +611,10 @@ class PagedKV:
         self._ref = [ctypes.addressof(d) for d in self._desc]
         self._lib, self._f32, self._norm_shape, self._scale = load(), torch.float32, (head_dim,), head_dim ** -0.5
 
+    def batch(self, page_table, q_start, kv_len, max_q_len: int) -> KVBatch:
+        """The sequences of a call on this cache (KVBatch)."""
+        return KVBatch(page_table, q_start, kv_len, max_q_len)
+
     def _rows(self, call: str, name: str, t, width: int, n: int = -1):
         """Checks a row tensor ([n, width] elements, rows any distance apart); its type id and row stride."""
         kind, shape, stride = self._types.get(t.dtype), t.shape, t.stride()

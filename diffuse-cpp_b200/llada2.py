@@ -17,6 +17,11 @@ for the block being denoised: the mask is block-causal, so a committed block's k
 depend on no later block, and MoE routing couples only the tokens of one routing block. The
 reference instead recomputes the whole window at every step. A block enters the cache in the
 first step of the next block, whose forward covers both blocks (block-causal mask between them).
+
+generate_batch keeps the keys and values of several sequences of unequal length in one paged cache
+(diffuse_moe.PagedKV, bf16, f16 or 8-bit pages) and denoises their current blocks together: QK norm,
+RoPE and the write into the pages are one kernel (dmoe_kv_append), attention over the pages another
+(dmoe_kv_attention), each reading what a sequence holds and no more.
 """
 from __future__ import annotations
 
@@ -225,6 +230,47 @@ class LLaDA2Model:
         return self._lin(x, "output")
 
 
+    def new_paged(self, n_pages: int, kv_type: str = "e4m3", page_size: int = 64) -> dm.PagedKV:
+        """A paged key/value cache for forward_paged: n_pages pages of page_size positions for every block."""
+        c = self.cfg
+        return dm.PagedKV(n_pages=n_pages, n_head_kv=c.n_head_kv, head_dim=c.head_dim, page_size=page_size,
+                          kv_type=kv_type, n_layer=c.n_layer, device=self.device)
+
+    def forward_paged(self, tokens: torch.Tensor, kv: dm.PagedKV, batch: dm.KVBatch,
+                      stream: Optional[int] = None) -> torch.Tensor:
+        """Logits [n, n_vocab] f32 of the batch's rows: `tokens` (int64 [n]) holds each sequence's last positions,
+        whole blocks of them, one sequence after the other (kv.batch(...)). Their keys and values are written into
+        the pages; each row attends to its sequence's positions up to the end of its own block. The same
+        as forward() of each sequence over its own cache, up to the pages' rounding."""
+        c = self.cfg
+        n = int(tokens.shape[0])
+        if n > self._max_n:
+            if self._graphs and n > self._graph_max_n:
+                self.drop_graphs()  # before the MoE layers grow under them
+            self._max_n = n
+        query_type = torch.float16 if kv.kv_type == "f16" else torch.bfloat16
+        y = torch.empty((n, c.n_embd), device=self.device, dtype=torch.float32)  # MoE outputs
+        x = self.w["tok_embd"][tokens].float()
+        for il in range(c.n_layer):
+            b = f"blk.{il}."
+            residual = x
+            h = rms_norm(x, self.w[b + "attn_norm"], c.rms_eps)
+            qkv = h.to(self.dtype) @ self.w[b + "attn_qkv"].t()
+            norms = (self.w[b + "attn_q_norm"], self.w[b + "attn_k_norm"]) if c.use_qk_norm else (None, None)
+            q = kv.append(il, qkv, batch, n_head=c.n_head, q_norm=norms[0], k_norm=norms[1], eps=c.rms_eps,
+                          rotary_dim=c.rotary_dim, rope_base=c.rope_base, q_type=query_type, stream=stream)
+            o = kv.attend(il, q, batch, block_length=c.block_length, stream=stream)
+            x = self._lin(o.view(n, -1), b + "attn_output") + residual
+            residual = x
+            h = rms_norm(x, self.w[b + "post_attn_norm"], c.rms_eps)
+            if il < c.first_k_dense:
+                x = self._lin(F.silu(self._lin(h, b + "ffn_gate")) * self._lin(h, b + "ffn_up"), b + "ffn_down") + residual
+            else:
+                self.moe[il].forward(h.contiguous(), out=y, stream=stream)
+                x = y + residual
+        return self._lin(rms_norm(x, self.w["output_norm"], c.rms_eps), "output")
+
+
 class _StepGraph:
     """One CUDA graph of LLaDA2Model.forward_static for n tokens over a fixed cache: fill `tokens`
     and `pos`, replay, read `logits`. Captured on first use after two eager runs of the same
@@ -264,7 +310,7 @@ def transfer_schedule(block_length: int, steps: int) -> list:
 
 
 def generate(model: LLaDA2Model, prompt: np.ndarray, n_generate: int, steps: int = 8, threshold: float = 0.95,
-             use_cache: bool = True, graphs: bool = False, sampler=None) -> tuple:
+             use_cache: bool = True, graphs: bool = False, sampler=None, kv_type: Optional[str] = None) -> tuple:
     """Greedy low-confidence block diffusion (generate_block_diffusion, diffuse-sampler.cpp:100-258):
     blocks tile from position 0; the prompt's whole blocks are prefilled; each later block runs up
     to `steps` denoising steps, each committing the schedule's count of its most confident masked
@@ -273,7 +319,13 @@ def generate(model: LLaDA2Model, prompt: np.ndarray, n_generate: int, steps: int
     at every step, as the reference does. graphs=True (with the cache) replays each step's forward
     from a CUDA graph, one per window size, kept by the model over the cache of model.reserve()
     (captured at first use, after the prefill). sampler: the step function with the signature of
-    diffuse_moe.sample_step (default: this library's GPU kernel)."""
+    diffuse_moe.sample_step (default: this library's GPU kernel). kv_type: "bf16", "f16" or "e4m3" for a
+    paged cache of that type instead (generate_batch of the one prompt; without graphs)."""
+    if kv_type is not None:
+        if graphs or not use_cache:
+            raise ValueError("a paged cache goes with use_cache=True and graphs=False")
+        seqs, forwards = generate_batch(model, [prompt], n_generate, steps, threshold, kv_type=kv_type, sampler=sampler)
+        return seqs[0], forwards
     sample = dm.sample_step if sampler is None else sampler
     c = model.cfg
     L = c.block_length
@@ -317,3 +369,89 @@ def generate(model: LLaDA2Model, prompt: np.ndarray, n_generate: int, steps: int
             sample(logits.contiguous(), blk_seq, c.mask_token_id, sched[step], threshold, token, prob, ncom)
             remaining -= int(ncom.item())
     return seq.cpu().numpy(), forwards
+
+
+def generate_batch(model: LLaDA2Model, prompts: list, n_generate: int, steps: int = 8, threshold: float = 0.95,
+                   kv_type: str = "e4m3", page_size: int = 64, kv=None, sampler=None) -> tuple:
+    """generate() for several prompts at once over one paged cache: every forward takes one denoising step of
+    each sequence that is not done, whatever their lengths and positions. Sequence i generates blocks until
+    n_generate positions past its prompt are covered, as generate() does. Returns the sequences (int32 numpy)
+    and the number of forwards. kv: a cache from model.new_paged() to use (its pages are taken from the first
+    on; default: a new one of kv_type). sampler: as for generate()."""
+    sample = dm.sample_step if sampler is None else sampler
+    c, dev = model.cfg, model.device
+    L = c.block_length
+    sched = transfer_schedule(L, min(steps, L))
+    n_blocks = [(len(p) + n_generate + L - 1) // L for p in prompts]
+    if kv is not None:
+        page_size = kv.page_size
+    pages = [-(-b * L // page_size) for b in n_blocks]
+    if kv is None:
+        kv = model.new_paged(max(1, sum(pages)), kv_type, page_size)
+    elif kv.n_pages < sum(pages):
+        raise ValueError(f"the sequences need {sum(pages)} pages, the cache has {kv.n_pages}")
+    tables = torch.full((len(prompts), max(pages, default=1)), -1, dtype=torch.int32)
+    at = 0
+    for i, m in enumerate(pages):
+        tables[i, :m] = torch.arange(at, at + m, dtype=torch.int32)
+        at += m
+    tables = tables.to(dev)
+    seqs = []
+    for p, b in zip(prompts, n_blocks):
+        s = torch.full((b * L,), c.mask_token_id, dtype=torch.int32, device=dev)
+        s[: len(p)] = torch.as_tensor(p, dtype=torch.int32, device=dev)
+        seqs.append(s)
+
+    def forward(which: list, rows: list) -> torch.Tensor:
+        """The logits of rows (begin, end) of each of the sequences `which`, one after the other."""
+        lens = [e - b for b, e in rows]
+        i32 = lambda v: torch.tensor(v, dtype=torch.int32).to(dev)  # noqa: E731
+        batch = kv.batch(tables[torch.tensor(which, device=dev)], i32([0] + list(np.cumsum(lens))),
+                         i32([e for _, e in rows]), max(lens))
+        return model.forward_paged(torch.cat([seqs[i][b:e] for i, (b, e) in zip(which, rows)]).long(), kv, batch)
+
+    # every whole prompt block but the last enters the cache at once
+    blk = [len(p) // L for p in prompts]
+    final = [max(0, b - 1) * L for b in blk]  # positions whose keys and values are final
+    forwards = 0
+    first = [i for i, f in enumerate(final) if f > 0]
+    if first:
+        forward(first, [(0, final[i]) for i in first])
+        forwards += 1
+    step = [0] * len(prompts)
+    left = [0] * len(prompts)
+
+    def open_block(i: int) -> None:
+        """Moves sequence i to its next block with masked positions, if there is one."""
+        step[i] = 0
+        while blk[i] < n_blocks[i]:
+            left[i] = int((seqs[i][blk[i] * L: (blk[i] + 1) * L] == c.mask_token_id).sum().item())
+            if left[i] or not sched:
+                return
+            blk[i] += 1
+
+    for i in range(len(prompts)):
+        open_block(i)
+    token = torch.empty((len(prompts), L), dtype=torch.int32, device=dev)
+    prob = torch.empty((len(prompts), L), dtype=torch.float32, device=dev)
+    ncom = torch.zeros(len(prompts), dtype=torch.int32, device=dev)
+    while True:
+        live = [i for i in range(len(prompts)) if blk[i] < n_blocks[i] and step[i] < len(sched)]
+        if not live:
+            return [s.cpu().numpy() for s in seqs], forwards
+        rows = [(final[i], (blk[i] + 1) * L) for i in live]  # the previous block, where it is new, and this one
+        logits = forward(live, rows)
+        forwards += 1
+        end = 0
+        for i, (b, e) in zip(live, rows):
+            end += e - b
+            sample(logits[end - L: end].contiguous(), seqs[i][e - L: e], c.mask_token_id, sched[step[i]], threshold,
+                   token[i], prob[i], ncom[i: i + 1])
+        done = ncom.tolist()
+        for i, (_, e) in zip(live, rows):
+            final[i] = e - L
+            left[i] -= done[i]
+            step[i] += 1
+            if left[i] == 0 or step[i] == len(sched):
+                blk[i] += 1
+                open_block(i)
