@@ -232,6 +232,19 @@ struct Walk {
   }
 };
 
+// mbar_wait by a whole warp, with one answer: after a timeout no lane goes on alone
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, uint32_t* err, uint32_t bit) {
+  const bool ok = mbar_wait(bar, parity, err, bit);
+  return __all_sync(0xffffffffu, ok);
+}
+
+// `bytes` (a multiple of 16, both addresses 16-byte aligned) into this CTA's shared memory
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
 // ---------------------------------------------------------------------------------------------
 // 16-bit warp products
 // ---------------------------------------------------------------------------------------------
@@ -336,23 +349,30 @@ __device__ __forceinline__ void store_lse(const AttnParams& p, int row0, int row
 // 16-byte loads. The order of the elements within a product's k is free as long as both sides agree:
 // for s it is the 16-byte chunk of a key row that a lane loads, for o the lane's value rows are joined
 // pairwise by byte permutations. p^T goes from accumulator to operand layout by an 8 x 8 transpose.
-// Bound by HBM: the bytes of the pages; each warp loads the next keys while it works on the values.
+// Bound by HBM: the bytes of the pages. A step's keys lie side by side in a page, and so do its values: each warp
+// has them brought into shared memory by one bulk copy each, one or two steps ahead (no barrier but the copies' own), so
+// that the latency of HBM does not show. A step's chain of dependent instructions is long, and only other warps
+// hide it: as many as registers and the ring leave room for.
 // ---------------------------------------------------------------------------------------------
 template <int HD, int KV, int NT>
 struct RowsCfg {
-  static constexpr int kWarps = 8;
+  static constexpr int kWarps = NT == 1 ? 12 : 8;  // registers: 168 or 255 a thread
   static constexpr int R = 8 * NT;
   static constexpr int MT = KV == KV_E4M3 ? 2 : 1;  // 16-position product tiles a step
   static constexpr int STEP = 16 * MT;
   static constexpr int TILE = kWarps * STEP;
-  static constexpr int OV = 1;
+  static constexpr int OV = 3;
   static constexpr int ES = KV == KV_E4M3 ? 1 : 2;
-  static constexpr size_t kSmem = (size_t)kWarps * R * (HD + 2) * 4;
+  static constexpr int kStages = kWarps == 8 ? 3 : 2;
+  static constexpr int kHalf = STEP * HD * ES;  // bytes of a step's keys, and of its values
+  static constexpr size_t kRing = (size_t)kWarps * kStages * 2 * kHalf;
+  static constexpr size_t kJoin = (size_t)kWarps * R * (HD + 2) * 4;
+  static constexpr size_t kSmem = kRing > kJoin ? kRing : kJoin;  // the ring is idle when the warps are joined
   static constexpr int kPart = R * (HD + 2);  // floats of a partial triple
 };
 
 template <int HD, int KV, int NT>
-__global__ void __launch_bounds__(256, 1) kv_rows_kernel(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(32 * RowsCfg<HD, KV, NT>::kWarps, 1) kv_rows_kernel(const __grid_constant__ AttnParams p) {
   using C = RowsCfg<HD, KV, NT>;
   constexpr bool kBf = KV == KV_BF16;
   constexpr int R = C::R, MT = C::MT, STEP = C::STEP, TILE = C::TILE, ES = C::ES;
@@ -360,14 +380,19 @@ __global__ void __launch_bounds__(256, 1) kv_rows_kernel(const __grid_constant__
   constexpr int VB = HD * ES / 8;          // bytes of a value row by each of 8 lanes: 8, 16 or 32
   constexpr int VW = VB / 4;
   constexpr int JT = HD / 16;              // 16-row tiles of o^T
-  extern __shared__ float smem_f[];
+  extern __shared__ __align__(128) float smem_f[];
   __shared__ int sums[C::kWarps];
   __shared__ Run found;
+  __shared__ uint64_t bar[C::kWarps][C::kStages];  // a stage's copies have arrived
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
 
+  if (lane < C::kStages) mbar_init(&bar[warp][lane], 1);
+  fence_mbar_init();
+  uint32_t done = 0;  // steps of the items before
+  bool ok = true;     // no wait has run out
   pdl_wait();
   Spanning begun = {-1, 0, 0, 0, 0, {0, 0, 0}};
-  for (Walk<R, TILE, C::OV> w(p, find_run<R, TILE, C::OV, 256>(p, sums, &found)); w.more(); w.next()) {
+  for (Walk<R, TILE, C::OV> w(p, find_run<R, TILE, C::OV, 32 * C::kWarps>(p, sums, &found)); w.more(); w.next()) {
     const Item& it = w.it;
     const int head = w.head;
     // queries: lane (g, t) holds row g of each 8-row tile, at the elements its key chunks cover
@@ -426,54 +451,68 @@ __global__ void __launch_bounds__(256, 1) kv_rows_kernel(const __grid_constant__
     const int end = (int)min((int64_t)lim_max, (int64_t)w.t1 * TILE);  // positions of this segment
     int pos = w.t0 * TILE + warp * STEP;
     const int32_t* table = p.b.table + it.seq * p.b.max_pages;
-    uint32_t kr[MT][2][KCH][4];
-    int64_t row = 0;
-    int ek = 0, ev = 0;
-    // page of a step's positions (a step lies in one scale block, so in one page), scales and keys
-    auto load_keys = [&](int at_pos) {
-      const uint32_t blk = (uint32_t)at_pos / kScaleBlock, slot = kv_slot(p.pg, blk);
-      int64_t page = table[slot];
-      if (page < 0 || page >= p.pg.n_pages) {
-        kv_report(p.pg.err, DMOE_KV_ERR_PAGE);
-        page = 0;
+    // first row and scales of the warp's next 32 steps, one a lane (a step lies in one scale block, so in one page)
+    const int steps = pos < end && ok ? (end - pos - 1) / (C::kWarps * STEP) + 1 : 0, pos_first = pos;
+    int64_t held_row = 0;
+    int held_scale = 0;
+    auto get_rows = [&](int first) {
+      const int at_pos = pos_first + (first + lane) * (C::kWarps * STEP);
+      if (first + lane < steps) {
+        const uint32_t blk = (uint32_t)at_pos / kScaleBlock, slot = kv_slot(p.pg, blk);
+        int64_t page = table[slot];
+        if (page < 0 || page >= p.pg.n_pages) {
+          kv_report(p.pg.err, DMOE_KV_ERR_PAGE);
+          page = 0;
+        }
+        held_row = kv_row(p.pg, page, head, (int)(blk - slot * p.pg.page_blocks) * kScaleBlock + at_pos % kScaleBlock);
+        if (KV == KV_E4M3) held_scale = p.pg.k_scale[held_row / kScaleBlock] | p.pg.v_scale[held_row / kScaleBlock] << 8;
       }
-      row = kv_row(p.pg, page, head, (int)(blk - slot * p.pg.page_blocks) * kScaleBlock + at_pos % kScaleBlock);
-      if (KV == KV_E4M3) {
-        ek = (int)p.pg.k_scale[row / kScaleBlock] - 127;
-        ev = (int)p.pg.v_scale[row / kScaleBlock] - 127;
+    };
+    uint8_t* const ring = reinterpret_cast<uint8_t*>(smem_f) + warp * (C::kStages * 2 * C::kHalf);
+    constexpr int VN = VB == 8 ? 1 : VB / 16;  // 16-byte pieces of a value row a lane
+    // Starts step n's copies; its scale bytes: key's, value's << 8.
+    auto issue = [&](int n) {
+      if (n >= steps) return 0;
+      if (n % 32 == 0) get_rows(n);
+      const int64_t row = __shfl_sync(0xffffffffu, held_row, n % 32);
+      const int sc = KV == KV_E4M3 ? __shfl_sync(0xffffffffu, held_scale, n % 32) : 0;
+      if (lane == 0) {
+        const uint32_t s = (done + n) % C::kStages;
+        uint8_t* const to = ring + s * 2 * C::kHalf;
+        mbar_arrive_expect_tx(&bar[warp][s], 2 * C::kHalf);
+        bulk_load(to, static_cast<const uint8_t*>(p.pg.k) + row * (HD * ES), C::kHalf, &bar[warp][s]);
+        bulk_load(to + C::kHalf, static_cast<const uint8_t*>(p.pg.v) + row * (HD * ES), C::kHalf, &bar[warp][s]);
       }
-      const uint8_t* base = static_cast<const uint8_t*>(p.pg.k) + row * (HD * ES);
+      return sc;
+    };
+    fence_proxy_async_smem();  // the ring was last written by the warps' joining
+    constexpr int kAhead = C::kStages - 1;
+    int scales[kAhead + 1];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) scales[i + 1] = issue(i);
+    int issued = min(steps, kAhead);
+    for (int n = 0; n < steps; ++n, pos += C::kWarps * STEP) {
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) scales[i] = scales[i + 1];
+      const int sc = scales[0];
+      __syncwarp();  // no lane needs anything of the step before
+      scales[kAhead] = issue(n + kAhead);
+      issued = min(steps, n + C::kStages);
+      const uint32_t stage = (done + n) % C::kStages;
+      ok = warp_wait(&bar[warp][stage], (done + n) / C::kStages & 1, p.wait_err, DMOE_KV_ERR_TIMEOUT);
+      if (!ok) break;
+      const uint32_t kat = smem_u32(ring + stage * 2 * C::kHalf) + g * (HD * ES) + 16 * t;
+      const uint32_t vat = smem_u32(ring + stage * 2 * C::kHalf + C::kHalf) + 2 * t * (HD * ES) + (VB == 8 ? 8 : 16) * g;
+      uint32_t kr[MT][2][KCH][4];
 #pragma unroll
       for (int a = 0; a < MT; ++a)
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int c = 0; c < KCH; ++c) {
-            const uint4 v = __ldcs(reinterpret_cast<const uint4*>(base + (16 * a + 8 * h + g) * (HD * ES) + 16 * (t + 4 * c)));
+            const uint4 v = lds128(kat + (16 * a + 8 * h) * (HD * ES) + 64 * c);
             kr[a][h][c][0] = v.x, kr[a][h][c][1] = v.y, kr[a][h][c][2] = v.z, kr[a][h][c][3] = v.w;
           }
-    };
-    if (pos < end) load_keys(pos);
-    for (; pos < end; pos += C::kWarps * STEP) {
-      // this step's values
-      uint32_t vr[MT][4][VW];
-      const uint8_t* vbase = static_cast<const uint8_t*>(p.pg.v) + row * (HD * ES);
-#pragma unroll
-      for (int a = 0; a < MT; ++a)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint8_t* src = vbase + (16 * a + 2 * t + (k & 1) + 8 * (k >> 1)) * (HD * ES);
-          if (VB == 8) {
-            const uint2 v = __ldcs(reinterpret_cast<const uint2*>(src + 8 * g));
-            vr[a][k][0] = v.x, vr[a][k][1] = v.y;
-          } else {
-#pragma unroll
-            for (int c = 0; c < VB / 16; ++c) {
-              const uint4 v = __ldcs(reinterpret_cast<const uint4*>(src + 16 * (g + 8 * c)));
-              vr[a][k][4 * c] = v.x, vr[a][k][4 * c + 1] = v.y, vr[a][k][4 * c + 2] = v.z, vr[a][k][4 * c + 3] = v.w;
-            }
-          }
-        }
       // s^T
       float s[NT][MT][4];
 #pragma unroll
@@ -494,11 +533,11 @@ __global__ void __launch_bounds__(256, 1) kv_rows_kernel(const __grid_constant__
           for (int n = 0; n < NT; ++n) mma16816<kBf>(s[n][a], af, qf[n][k][0], qf[n][k][1]);
         }
       }
-      const float sk = KV == KV_E4M3 ? pow2i(ek) : 1.f, evf = KV == KV_E4M3 ? (float)ev : 0.f;
+      const int ev = KV == KV_E4M3 ? (sc >> 8) - 127 : 0;
+      const float sk = KV == KV_E4M3 ? pow2i((sc & 255) - 127) : 1.f, evf = (float)ev;
       const float unv = KV == KV_E4M3 ? pow2i(-ev) : 1.f;
       const int here = pos;
       const bool edge = here + STEP > lim_min;
-      if (pos + C::kWarps * STEP < end) load_keys(pos + C::kWarps * STEP);  // the next step's keys
 
       // scores -> weights. Lane (g, t): positions 16a + g and 16a + 8 + g, rows 2t and 2t + 1
       uint32_t pf[NT][MT][2];
@@ -552,6 +591,22 @@ __global__ void __launch_bounds__(256, 1) kv_rows_kernel(const __grid_constant__
             for (int i = 0; i < 4; ++i) o[n][j][i] *= shrink[i & 1];
         }
       }
+      uint32_t vr[MT][4][VW];
+#pragma unroll
+      for (int a = 0; a < MT; ++a)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t at = vat + (16 * a + (k & 1) + 8 * (k >> 1)) * (HD * ES);
+          if (VB == 8) {
+            asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(vr[a][k][0]), "=r"(vr[a][k][1]) : "r"(at));
+          } else {
+#pragma unroll
+            for (int c = 0; c < VN; ++c) {
+              const uint4 v = lds128(at + 128 * c);
+              vr[a][k][4 * c] = v.x, vr[a][k][4 * c + 1] = v.y, vr[a][k][4 * c + 2] = v.z, vr[a][k][4 * c + 3] = v.w;
+            }
+          }
+        }
       if (edge) {
         // positions past the sequence's end hold anything: their weights are zero, so must be the values
 #pragma unroll
@@ -625,7 +680,13 @@ __global__ void __launch_bounds__(256, 1) kv_rows_kernel(const __grid_constant__
         }
     }
 
+    // after a timeout: what is still on its way (with the same limit), then on to the end
+    if (!ok)
+      for (int n = 0; n < issued; ++n) warp_wait(&bar[warp][(done + n) % C::kStages], (done + n) / C::kStages & 1, p.wait_err, DMOE_KV_ERR_TIMEOUT);
+    done += steps;
+
     // join the warps: o, M and the sum of each row
+    __syncthreads();  // every warp has left the ring
     float* os = smem_f;                           // [warp][row][d]
     float* ml = smem_f + C::kWarps * R * HD;      // [warp][row][2]
 #pragma unroll
@@ -650,7 +711,7 @@ __global__ void __launch_bounds__(256, 1) kv_rows_kernel(const __grid_constant__
     __syncthreads();
     const bool whole = w.whole();
     float* part = p.part + (int64_t)(2 * blockIdx.x + (w.t0 == 0 ? 1 : 0)) * C::kPart;
-    for (int i = tid; i < it.rows * HD; i += 256) {
+    for (int i = tid; i < it.rows * HD; i += 32 * C::kWarps) {
       const int r = i / HD, d = i % HD;
       float mm = -INFINITY;
 #pragma unroll
@@ -711,11 +772,6 @@ struct TileBars {
   uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], read[4], reset, done;
 };
 
-// mbar_wait by a whole warp, with one answer: after a timeout no lane goes on alone
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, uint32_t* err, uint32_t bit) {
-  const bool ok = mbar_wait(bar, parity, err, bit);
-  return __all_sync(0xffffffffu, ok);
-}
 
 template <int HD, int KV>
 __global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__ AttnParams p) {
@@ -1511,7 +1567,7 @@ cudaError_t launch_rows(AttnParams p, int max_rows, cudaStream_t st) {
   p.n_qt = (max_rows + C::R - 1) / C::R;
   static_assert(C::kSmem <= 227 * 1024, "shared memory");
   cudaError_t e = allow_smem(kv_rows_kernel<HD, KV, NT>, C::kSmem, seen);
-  if (e == cudaSuccess) e = launch_pdl(kv_rows_kernel<HD, KV, NT>, dim3(kRowsGrid), dim3(256), C::kSmem, st, p);
+  if (e == cudaSuccess) e = launch_pdl(kv_rows_kernel<HD, KV, NT>, dim3(kRowsGrid), dim3(32 * C::kWarps), C::kSmem, st, p);
   if (e == cudaSuccess) e = launch_pdl(kv_combine_kernel<HD, C::R>, dim3(kCombineGrid), dim3(256), 0, st, p, kRowsGrid);
   return e;
 }
