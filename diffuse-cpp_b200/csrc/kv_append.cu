@@ -208,7 +208,7 @@ __device__ __forceinline__ void dequantise8(uint2 w, float scale, float (&x)[8])
 }
 
 template <int HD, int KV, int IN>
-__global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_constant__ AppendParams p) {
+__global__ void __launch_bounds__(kThreads, 4) kv_append_kernel(const __grid_constant__ AppendParams p) {
   constexpr int LPR = HD / 8;     // lanes a row
   constexpr int RPW = 32 / LPR;   // rows a warp holds at once
   constexpr int PASSES = kScaleBlock / (kWarps * RPW);

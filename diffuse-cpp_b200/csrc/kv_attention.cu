@@ -53,6 +53,7 @@ struct AttnParams {
   uint32_t group_magic;  // ceil(2^28 / group): x / group for x < 2^13 and group <= 2^12 (x * error < 2^28)
   int block_length;
   int n_qt;          // row tiles a sequence can have (max_q_len)
+  int whole;         // items are not split: no partial triples, no second kernel
   int vec_q, vec_q16, vec_out16;  // q rows allow 8-byte, 16-byte loads; out rows 16-byte stores
   float scale_log2;  // scale * log2(e)
   uint32_t* wait_err;  // word that bounded waits report to
@@ -122,7 +123,7 @@ __device__ __forceinline__ Item item_of(const AttnParams& p, int u) {
 }
 
 // Beginning and ending an item costs about as much as OV tiles. An item of t tiles is OV + t units long, and
-// the units of all items are numbered through; its tiles are the last t.
+// the units of all items are numbered through; its tiles are the last t. With p.whole an item is one unit.
 // The host refuses calls whose units could number 2^31 or more.
 struct Run {   // a CTA's run of units
   Item it;     // first item
@@ -143,7 +144,7 @@ __device__ __forceinline__ Run find_run(const AttnParams& p, int* sums, Run* fou
   int mine = 0;
   for (int u = u0; u < u1; ++u) {
     const int t = item_of<R, TILE>(p, u).tiles;
-    if (t) mine += t + OV;
+    if (t) mine += p.whole ? 1 : t + OV;
   }
   int incl = mine;
 #pragma unroll
@@ -167,7 +168,7 @@ __device__ __forceinline__ Run find_run(const AttnParams& p, int* sums, Run* fou
   if (first < total && first >= before && first < before + mine * heads) {
     for (int u = u0; u < u1; ++u) {
       const Item it = item_of<R, TILE>(p, u);
-      const int w = it.tiles ? it.tiles + OV : 0;
+      const int w = !it.tiles ? 0 : p.whole ? 1 : it.tiles + OV;
       if (first < before + w * heads) {
         found->it = it;
         found->u = u;
@@ -211,7 +212,7 @@ struct Walk {
 
  private:
   __device__ __forceinline__ void advance() {
-    const int n = min(left, OV + it.tiles - unit);
+    const int n = p.whole ? 1 : min(left, OV + it.tiles - unit);
     left -= n;
     at += n;
     unit = 0;
@@ -223,8 +224,8 @@ struct Walk {
   }
   __device__ __forceinline__ void settle() {
     while (left > 0) {
-      t0 = max(0, unit - OV);
-      t1 = min(it.tiles, unit + left - OV);
+      t0 = p.whole ? 0 : max(0, unit - OV);
+      t1 = p.whole ? it.tiles : min(it.tiles, unit + left - OV);
       if (t1 > t0) break;
       advance();
     }
@@ -395,47 +396,7 @@ __global__ void __launch_bounds__(32 * RowsCfg<HD, KV, NT>::kWarps, 1) kv_rows_k
   for (Walk<R, TILE, C::OV> w(p, find_run<R, TILE, C::OV, 32 * C::kWarps>(p, sums, &found)); w.more(); w.next()) {
     const Item& it = w.it;
     const int head = w.head;
-    // queries: lane (g, t) holds row g of each 8-row tile, at the elements its key chunks cover
-    uint32_t qf[NT][HD / 16][2];
-    float cq[NT][2];  // score factor and limit of the rows 2t, 2t + 1 of each tile
-    int lim[NT][2];
-    int lim_min = INT32_MAX, lim_max = 0;
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int row = it.row_lo + n * 8 + g;
-      const bool live = n * 8 + g < it.rows;
-      float x[HD / 16][4];
-      float amax = 0.f;
-#pragma unroll
-      for (int k = 0; k < HD / 16; ++k) {
-        const int d = ES == 1 ? 16 * (t + 4 * (k / 4)) + 4 * (k % 4) : 8 * (t + 4 * (k / 2)) + 4 * (k % 2);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[k][i] = 0.f;
-        if (live)
-          load_q4(p, (int64_t)(it.q.row0 + row / p.group) * p.q_stride + (int64_t)(head * p.group + row % p.group) * HD + d, x[k]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) amax = fmaxf(amax, fabsf(x[k][i]));
-      }
-      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-      // f16 products: rows scaled into [-1, 1]
-      const int e = kBf ? 0 : min(max((int)(__float_as_uint(amax) >> 23) - 126, -100), 100);
-      const float inv = pow2i(-e);
-#pragma unroll
-      for (int k = 0; k < HD / 16; ++k) {
-        qf[n][k][0] = pack2<kBf>(x[k][0] * inv, x[k][1] * inv);
-        qf[n][k][1] = pack2<kBf>(x[k][2] * inv, x[k][3] * inv);
-      }
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int r = n * 8 + 2 * t + i;
-        cq[n][i] = p.scale_log2 * pow2i(__shfl_sync(0xffffffffu, e, (2 * t + i) * 4));
-        lim[n][i] = r < it.rows ? row_limit(p, it.q, it.row_lo + r) : 0;
-      }
-    }
-    lim_min = row_limit(p, it.q, it.row_lo);
-    lim_max = row_limit(p, it.q, it.row_lo + it.rows - 1);
-
+    const int lim_min = row_limit(p, it.q, it.row_lo), lim_max = row_limit(p, it.q, it.row_lo + it.rows - 1);
     float o[NT][JT][4];
     float m[NT][2], l[NT][2];
 #pragma unroll
@@ -475,7 +436,6 @@ __global__ void __launch_bounds__(32 * RowsCfg<HD, KV, NT>::kWarps, 1) kv_rows_k
       if (n >= steps) return 0;
       if (n % 32 == 0) get_rows(n);
       const int64_t row = __shfl_sync(0xffffffffu, held_row, n % 32);
-      const int sc = KV == KV_E4M3 ? __shfl_sync(0xffffffffu, held_scale, n % 32) : 0;
       if (lane == 0) {
         const uint32_t s = (done + n) % C::kStages;
         uint8_t* const to = ring + s * 2 * C::kHalf;
@@ -483,7 +443,7 @@ __global__ void __launch_bounds__(32 * RowsCfg<HD, KV, NT>::kWarps, 1) kv_rows_k
         bulk_load(to, static_cast<const uint8_t*>(p.pg.k) + row * (HD * ES), C::kHalf, &bar[warp][s]);
         bulk_load(to + C::kHalf, static_cast<const uint8_t*>(p.pg.v) + row * (HD * ES), C::kHalf, &bar[warp][s]);
       }
-      return sc;
+      return KV == KV_E4M3 ? __shfl_sync(0xffffffffu, held_scale, n % 32) : 0;
     };
     fence_proxy_async_smem();  // the ring was last written by the warps' joining
     constexpr int kAhead = C::kStages - 1;
@@ -491,6 +451,43 @@ __global__ void __launch_bounds__(32 * RowsCfg<HD, KV, NT>::kWarps, 1) kv_rows_k
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) scales[i + 1] = issue(i);
     int issued = min(steps, kAhead);
+    // queries: lane (g, t) holds row g of each 8-row tile, at the elements its key chunks cover
+    uint32_t qf[NT][HD / 16][2];
+    float cq[NT][2];  // score factor and limit of the rows 2t, 2t + 1 of each tile
+    int lim[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int row = it.row_lo + n * 8 + g;
+      const bool live = n * 8 + g < it.rows;
+      float x[HD / 16][4];
+      float amax = 0.f;
+#pragma unroll
+      for (int k = 0; k < HD / 16; ++k) {
+        const int d = ES == 1 ? 16 * (t + 4 * (k / 4)) + 4 * (k % 4) : 8 * (t + 4 * (k / 2)) + 4 * (k % 2);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[k][i] = 0.f;
+        if (live)
+          load_q4(p, (int64_t)(it.q.row0 + row / p.group) * p.q_stride + (int64_t)(head * p.group + row % p.group) * HD + d, x[k]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) amax = fmaxf(amax, fabsf(x[k][i]));
+      }
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+      // f16 products: rows scaled into [-1, 1]
+      const int e = kBf ? 0 : min(max((int)(__float_as_uint(amax) >> 23) - 126, -100), 100);
+      const float inv = pow2i(-e);
+#pragma unroll
+      for (int k = 0; k < HD / 16; ++k) {
+        qf[n][k][0] = pack2<kBf>(x[k][0] * inv, x[k][1] * inv);
+        qf[n][k][1] = pack2<kBf>(x[k][2] * inv, x[k][3] * inv);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = n * 8 + 2 * t + i;
+        cq[n][i] = p.scale_log2 * pow2i(__shfl_sync(0xffffffffu, e, (2 * t + i) * 4));
+        lim[n][i] = r < it.rows ? row_limit(p, it.q, it.row_lo + r) : 0;
+      }
+    }
     for (int n = 0; n < steps; ++n, pos += C::kWarps * STEP) {
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) scales[i] = scales[i + 1];
@@ -1547,6 +1544,10 @@ __global__ void __launch_bounds__(256) kv_combine_tiles_kernel(const __grid_cons
 constexpr int kRowsGrid = kMaxGrid;
 constexpr int kTileGrid = kMaxGrid;
 constexpr int kCombineGrid = 8 * kMaxGrid;
+// Items are not split over CTAs, which saves the partial triples and the second kernel, where an item can have at
+// most kWholeTiles tiles (one sequence, 500 positions: 12.0 us against 13.8 split; at 6 tiles 19.7 against 13.8), or
+// kWholeTilesMany where there are kMany items or more (64 sequences of 2200 positions: 43.7 against 48.6 us).
+constexpr int kWholeTiles = 3, kWholeTilesMany = 8, kMany = 64;
 constexpr int kRowsMax = 16;  // rows of a sequence and key/value head that the few-rows kernel takes
 
 // The shared memory limit of a kernel, raised once on each device.
@@ -1565,10 +1566,11 @@ cudaError_t launch_rows(AttnParams p, int max_rows, cudaStream_t st) {
   using C = RowsCfg<HD, KV, NT>;
   static std::atomic<uint64_t> seen{0};
   p.n_qt = (max_rows + C::R - 1) / C::R;
+  p.whole = p.b.max_pages * p.pg.page_size <= (p.b.n_seq * p.pg.n_head_kv >= kMany ? kWholeTilesMany : kWholeTiles) * C::TILE;
   static_assert(C::kSmem <= 227 * 1024, "shared memory");
   cudaError_t e = allow_smem(kv_rows_kernel<HD, KV, NT>, C::kSmem, seen);
   if (e == cudaSuccess) e = launch_pdl(kv_rows_kernel<HD, KV, NT>, dim3(kRowsGrid), dim3(32 * C::kWarps), C::kSmem, st, p);
-  if (e == cudaSuccess) e = launch_pdl(kv_combine_kernel<HD, C::R>, dim3(kCombineGrid), dim3(256), 0, st, p, kRowsGrid);
+  if (e == cudaSuccess && !p.whole) e = launch_pdl(kv_combine_kernel<HD, C::R>, dim3(kCombineGrid), dim3(256), 0, st, p, kRowsGrid);
   return e;
 }
 
@@ -1577,10 +1579,11 @@ cudaError_t launch_tiles(AttnParams p, int max_rows, cudaStream_t st) {
   using C = TileCfg<HD, KV>;
   static std::atomic<uint64_t> seen{0};
   p.n_qt = (max_rows + C::R - 1) / C::R;
+  p.whole = p.b.max_pages * p.pg.page_size <= (p.b.n_seq * p.pg.n_head_kv >= kMany ? kWholeTilesMany : kWholeTiles) * C::TILE;
   static_assert(C::kSmem <= 220 * 1024, "shared memory");
   cudaError_t e = allow_smem(kv_tile_kernel<HD, KV>, C::kSmem, seen);
   if (e == cudaSuccess) e = launch_pdl(kv_tile_kernel<HD, KV>, dim3(kTileGrid), dim3(C::kThreads), C::kSmem, st, p);
-  if (e == cudaSuccess) e = launch_pdl(kv_combine_tiles_kernel<HD, C::R>, dim3(kCombineGrid), dim3(256), 0, st, p, kTileGrid);
+  if (e == cudaSuccess && !p.whole) e = launch_pdl(kv_combine_tiles_kernel<HD, C::R>, dim3(kCombineGrid), dim3(256), 0, st, p, kTileGrid);
   return e;
 }
 
