@@ -44,6 +44,7 @@ struct AppendParams {
   int q_type;
   int n_head;
   int half;          // rotary_dim / 2
+  uint32_t half_magic;  // ceil(2^18 / half): i / half for i < 2^11 (i * error < 2^11 * 2^6)
   int flat_slots;    // heads of the independent rows: [0, flat_slots)
   int flat_per_cta, flat_groups;  // heads a CTA takes of them, and how many such groups
   int held_per_cta, held_groups;  // the same of the key heads, and of the value heads, of 8-bit pages
@@ -150,7 +151,7 @@ __device__ __forceinline__ void norm_rotate(float (&x)[8], const float (&w)[8], 
   for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
 #pragma unroll
   for (int o = LPR / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  const float r = norm ? 1.0f / sqrtf(ss * (1.0f / (8 * LPR)) + eps) : 1.0f;
+  const float r = norm ? rsqrtf(fmaf(ss, 1.0f / (8 * LPR), eps)) : 1.0f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] *= r * w[i];
   if (half == 0) return;
@@ -266,7 +267,7 @@ __global__ void __launch_bounds__(kThreads, 4) kv_append_kernel(const __grid_con
   // (cos, sin) of the block's new positions, once for all heads of the CTA; values are not rotated
   const bool values = group >= p.flat_groups + p.held_groups;
   for (int i = tid; i < (values ? 0 : fresh * p.half); i += kThreads) {
-    const int t = i / p.half, f = i % p.half;
+    const int t = (int)((i * p.half_magic) >> 18), f = i - t * p.half;
     const double a = (double)(lo + t) * p.turns[f];
     float sn, c;
     sincospif(2.0f * (float)(a - rint(a)), &sn, &c);
@@ -318,7 +319,7 @@ __global__ void __launch_bounds__(kThreads, 4) kv_append_kernel(const __grid_con
         const float2* const c = cs + (lo - b0 + t) * kMaxHalf;
         if (KV == KV_E4M3) {
           norm_rotate<LPR>(y, wq, p.q_norm != nullptr, p.eps, sub, p.half, c);
-        } else {
+        } else if (!__all_sync(0xffffffffu, is_v || !live)) {
           float w[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) w[i] = is_q ? wq[i] : wk[i];
@@ -503,14 +504,17 @@ extern "C" dmoe_status dmoe_kv_append(const dmoe_kv_cache* cache, const dmoe_kv_
   p.vec_in = aligned16(a->qkv, a->qkv_stride * size_of(a->qkv_type));
   p.vec_out = aligned16(a->q_out, a->q_stride * size_of(a->q_type));
   if (p.half > 0) {
+    p.half_magic = ((1u << 18) + p.half - 1) / p.half;
     // base^(-2i / r) as powers of one ratio: 63 products of 64 bits stay within 1e-14 of the power
     const double ratio = pow(a->rope_base, -2.0 / a->rotary_dim);
     double t = 0.15915494309189533577;  // 1 / 2 pi
     for (int i = 0; i < p.half; ++i, t *= ratio) p.turns[i] = t;
   }
   const KvType kv = kv_type_of(cache->type);
-  // a sequence of f new rows touches at most f blocks, and at most f / 32 + 2
-  const int64_t units = std::min<int64_t>(a->n_tokens, a->n_tokens / kScaleBlock + 2ll * batch->n_seq);
+  // a sequence of f rows touches at most f blocks, at most f / 32 + 2, and at most (f + 62) / 32
+  const int64_t units = std::min<int64_t>({a->n_tokens, a->n_tokens / kScaleBlock + 2ll * batch->n_seq,
+                                  ((int64_t)batch->max_q_len + 2 * kScaleBlock - 2) / kScaleBlock * batch->n_seq});
+  if (units == 0) return DMOE_OK;
   const bool held = kv == KV_E4M3;
   p.flat_slots = a->n_head + (held ? 0 : 2 * nk);
   // Heads a CTA takes: as many as leave about kWanted CTAs (the rotation's table is then made for several heads; one
