@@ -766,7 +766,7 @@ struct TileCfg {
 };
 
 struct TileBars {
-  uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], read[4], reset, done;
+  uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_part[2], p_full[2], o_full[2], read[4], reset, done;
 };
 
 
@@ -804,6 +804,7 @@ __global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__
       mbar_init(&bar.v_full[i], C::kLoaders);
       mbar_init(&bar.v_empty[i], 1);
       mbar_init(&bar.s_full[i], 1);
+      mbar_init(&bar.p_part[i], 128);
       mbar_init(&bar.p_full[i], 128);
       mbar_init(&bar.o_full[i], 1);
     }
@@ -843,12 +844,12 @@ __global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__
           }
           mma_commit(&bar.s_full[half]);
         };
-        auto outputs = [&](int half, int stage, bool first) {
-          const uint64_t vd = v_desc + stage * (C::kOperand / 16);
-          mma_f16_ts(tmem + 256 + half * 128, tmem + half * 128, vd, kIdescO, !first);
+        auto outputs = [&](int half, int stage, int part, bool first) {
+          const uint64_t vd = v_desc + stage * (C::kOperand / 16) + part * 4 * (2048 / 16);
+          const uint32_t pa = tmem + half * 128 + part * 32;
+          mma_f16_ts(tmem + 256 + half * 128, pa, vd, kIdescO, !first);
 #pragma unroll
-          for (int k = 1; k < TILE / 16; ++k)
-            mma_f16_ts(tmem + 256 + half * 128, tmem + half * 128 + 8 * k, vd + k * (2048 / 16), kIdescO, 1);
+          for (int k = 1; k < TILE / 32; ++k) mma_f16_ts(tmem + 256 + half * 128, pa + 8 * k, vd + k * (2048 / 16), kIdescO, 1);
         };
         for (; ok && w.more(); w.next()) {
           const int halves = w.it.rows > 128 ? 2 : 1, tiles = w.t1 - w.t0;
@@ -861,11 +862,15 @@ __global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__
             const int stage = n & 1, next = (n + 1) & 1;
             ok = wait(&bar.v_full[stage], (n >> 1) & 1);
             for (int h = 0; ok && h < halves; ++h) {
+              ok = wait(&bar.p_part[h], ph_p[h]);
+              if (!ok) break;
+              tc_fence_after();
+              outputs(h, stage, 0, j == 0);
               ok = wait(&bar.p_full[h], ph_p[h]);
               if (!ok) break;
               ph_p[h] ^= 1;
               tc_fence_after();
-              outputs(h, stage, j == 0);
+              outputs(h, stage, 1, false);
               if (h == halves - 1) mma_commit(&bar.v_empty[stage]);
               if (j + 1 < tiles) {
                 if (h == 0) {
@@ -1265,6 +1270,11 @@ __global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__
           float a, d;
           unpair(add2(sum[0], sum[1]), a, d);
           l = fmaf(a + d, un[b], l);
+          if (b == 1) {  // the products of the first half of the columns need not wait
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(&bar.p_part[half]);
+          }
         }
         tmem_wait_st();
         tc_fence_before();
