@@ -783,8 +783,9 @@ __global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__
   __shared__ Run found;
   __shared__ int not_finite_from[4][HD];  // [item of the run & 3][d]: first position whose value is not finite
   __shared__ int any_not_finite[4];
-  // scales of keys, exponents of values and their reciprocal scales [..][tile of the run & 3][32-position block]. Written before the tile's arrival; the
-  // slot is free again when the tile two on has been multiplied by both halves' queries
+  // scales of keys, exponents of values and their reciprocal scales [..][tile of the run & 3][32-position block].
+  // Written with the keys, before their arrival; the slot is free again when the tile two on has been multiplied by
+  // the queries of both halves
   __shared__ __align__(16) float scale_s[3][4][4];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* q_s = smem;                                 // [half] operands
@@ -793,6 +794,9 @@ __global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__
   uint8_t* out_s = v_s + C::kStages * C::kOperand;     // [softmax warp]
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
+  // tensor memory only after the kernel before has ended: one that still had to allocate its own would wait for
+  // this one, which waits for it
+  pdl_wait();
   if (warp == 16) {
     tmem_alloc(&tmem_base_s, 512);
     tmem_relinquish();
@@ -816,7 +820,6 @@ __global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__
   }
   if (tid < 4) any_not_finite[tid] = 0;
   tc_fence_before();
-  pdl_wait();
   const Run run = find_run<R, TILE, C::OV, C::kThreads>(p, sums, &found);  // ends with a barrier of the CTA
   tc_fence_after();
   const uint32_t tmem = tmem_base_s;
@@ -951,11 +954,11 @@ __global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__
     };
     auto limit = [&]() { return row_limit(p, w.it.q, w.it.row_lo + w.it.rows - 1); };
     uint4 x[KV == KV_E4M3 ? N : 1];  // 8-bit pages: the next tile, on its way
-    int scale = 0;                   // and the exponent of its block `lane` (threads 0-3)
+    int scale = 0;                   // and the scale bytes of its block `lane`: key's, value's << 8 (key loaders 0-3)
     auto fetch = [&](int tile, int lim) {
       if constexpr (KV == KV_E4M3) {
-        scale = 0;
-        if (lt < 4 && tile * TILE + 32 * lt < lim) scale = (int)(is_v ? p.pg.v_scale : p.pg.k_scale)[scale_at] - 127;
+        scale = 127 | 127 << 8;
+        if (!is_v && lt < 4 && tile * TILE + 32 * lt < lim) scale = p.pg.k_scale[scale_at] | p.pg.v_scale[scale_at] << 8;
         if ((tile + 1) * TILE <= lim) {
 #pragma unroll
           for (int i = 0; i < N; ++i) x[i] = __ldg(reinterpret_cast<const uint4*>(source(i)));
@@ -985,11 +988,10 @@ __global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__
         if (!ok) break;
         const bool edge = is_v && lim_min < lim_max && (t + 1) * TILE > lim_min;
         if constexpr (KV == KV_E4M3) {
-          if (lt < 4) {
-            if (is_v)
-              scale_s[1][n & 3][lt] = (float)scale, scale_s[2][n & 3][lt] = pow2i(-scale);
-            else
-              scale_s[0][n & 3][lt] = pow2i(scale);
+          // the values' scales too: the softmax needs them with the scores, before the values need be here
+          if (!is_v && lt < 4) {
+            const int ev = (scale >> 8) - 127;
+            scale_s[0][n & 3][lt] = pow2i((scale & 255) - 127), scale_s[1][n & 3][lt] = (float)ev, scale_s[2][n & 3][lt] = pow2i(-ev);
           }
           if (edge) {
 #pragma unroll
@@ -1163,6 +1165,9 @@ __global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__
       const float factor = next_factor;
       if (!whole && w.t0 == 0) begun = w.begun();
       if (!active) {
+        // not ahead of the other half: an arrival for the next item would count for this one's queries
+        ok = warp_wait(&bar.q_full, seg & 1, err, kTimeout);
+        if (!ok) break;
         mbar_arrive(&bar.read[seg & 3]);
         n += w.t1 - w.t0;
         w.next();

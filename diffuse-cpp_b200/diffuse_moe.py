@@ -628,6 +628,15 @@ class PagedKV:
             raise ValueError(f"{call}: {name} must hold {'n' if n < 0 else n} rows of {width} consecutive elements")
         return kind, stride[0] if shape[0] > 1 else max(width, stride[0])
 
+    def _empty(self, like, shape, dtype, stream):
+        """A new tensor of the pool of the launching stream."""
+        if stream is None:
+            return like.new_empty(shape, dtype=dtype)
+        import torch
+
+        with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=self.device)):
+            return like.new_empty(shape, dtype=dtype)
+
     def _launch(self, batch: KVBatch, stream, fn, *args):
         """fn(stream, *args) with the cache's device current; `stream` None: the current torch stream."""
         import torch
@@ -650,7 +659,7 @@ class PagedKV:
         kind, stride = self._rows("append", "qkv", qkv, (n_head + 2 * self.n_head_kv) * self.head_dim)
         n = qkv.shape[0]
         if q_out is None:
-            q_out = qkv.new_empty((n, n_head, self.head_dim), dtype=q_type)
+            q_out = self._empty(qkv, (n, n_head, self.head_dim), q_type, stream)
         q_kind, q_stride = self._rows("append", "q_out", q_out, n_head * self.head_dim, n)
         for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
             if w is not None and (w.shape != self._norm_shape or w.dtype != self._f32 or w.device != self.device
@@ -675,7 +684,7 @@ class PagedKV:
         n, n_head, _ = q.shape
         kind, stride = self._rows("attend", "q", q, n_head * self.head_dim)
         if out is None:
-            out = q.new_empty(q.shape)
+            out = self._empty(q, q.shape, None, stream)
         o_kind, o_stride = self._rows("attend", "out", out, n_head * self.head_dim, n)
         if o_kind != kind:
             raise ValueError("attend: out must have q's type")
@@ -692,14 +701,8 @@ class PagedKV:
         size = self._lib.dmoe_kv_attention_workspace(cache, batch._ref, args)
         if not size:
             return self._lib.dmoe_kv_attention(cache, batch._ref, args, None, 0, stream)
-        # of the launching stream's pool: calls on different streams and in different graphs have their own
-        if given is None:
-            ws = self.err.new_empty(size // 4)
-        else:
-            import torch
-
-            with torch.cuda.stream(torch.cuda.ExternalStream(given, device=self.device)):
-                ws = self.err.new_empty(size // 4)
+        # calls on different streams and in different graphs have workspaces of their own
+        ws = self._empty(self.err, (size // 4,), None, given)
         return self._lib.dmoe_kv_attention(cache, batch._ref, args, ws.data_ptr(), size, stream)
 
     def check(self) -> None:

@@ -334,8 +334,8 @@ typedef struct dmoe_kv_cache {
  * kv_len[s] - q_len + i. Rows at negative positions (a batch padded on the left) are padding: they
  * enter no cache, and their outputs are zero. Rows behind q_start[n_seq] are not touched.
  * Position p lies in page page_table[s][p / page_size] at p % page_size; entries past kv_len are not
- * read. Pages that a call writes must belong to one sequence; pages that are only read may be
- * shared. max_q_len is an upper bound of the rows of a sequence. */
+ * read. A page that a call writes must stand in one place of the table only; pages that are only read
+ * may be shared. max_q_len is an upper bound of the rows of a sequence. */
 typedef struct dmoe_kv_batch {
   const int32_t* page_table; /* DEVICE, [n_seq][max_pages] */
   const int32_t* q_start;    /* DEVICE, [n_seq + 1] */
@@ -356,7 +356,7 @@ typedef struct dmoe_kv_batch {
 typedef struct dmoe_kv_append_args {
   const void* qkv;
   void* q_out;          /* [n_tokens][n_head][head_dim] */
-  const float* q_norm;  /* [head_dim] or NULL */
+  const float* q_norm;  /* [head_dim], 16-byte aligned, or NULL */
   const float* k_norm;
   int64_t n_tokens;
   int64_t qkv_stride;   /* elements between rows */

@@ -283,6 +283,87 @@ def test_attend_graph_stream_and_repeat(rows):
     s.kv.check()
 
 
+def gpu_values(s, which, i, n):
+    """held() as a float64 tensor on the GPU [n, heads_kv, d]."""
+    t = getattr(s.kv, which)[0]
+    p = torch.arange(n, device="cuda")
+    pg, of = torch.from_numpy(s.table[i].astype(np.int64)).cuda()[p // s.page], p % s.page
+    if s.kv_name != "e4m3":
+        return t[pg, :, of].double()
+    sc = getattr(s.kv, which + "_scale")[0].view(torch.uint8)[pg, :, of // 32].double()
+    return t.view(torch.uint8)[pg, :, of].view(torch.float8_e4m3fn).double() * torch.exp2(sc - 127)[..., None]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv,q_len,block,io", [("e4m3", 32, 32, "bf16"), ("e4m3", 33, 1, "f16"), ("bf16", 32, 32, "bf16"),
+                                               ("e4m3", 1, 1, "bf16"), ("f16", 2, 1, "f16")])
+def test_attend_whole_batches_with_cold_caches(kv, q_len, block, io):
+    """Batches that fill the GPU, every row of the output, with keys and values from memory and not from L2:
+    whatever the kernel's parts are handed late must still be there when it is used."""
+    s = Setup([q_len] * 12, [9000 - 600 * i + (i % 3) for i in range(12)], kv, 32, 4, 128, page=64, seed=q_len)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    for held, scale in ((s.kv.k, s.kv.k_scale), (s.kv.v, s.kv.v_scale)):
+        x = torch.randn(held.shape, generator=g, device="cuda")
+        held.copy_(x.to(held.dtype))
+        if kv == "e4m3":  # scales that differ from block to block
+            scale.view(torch.uint8).copy_(torch.randint(121, 128, scale.shape, generator=g, device="cuda").to(torch.uint8))
+    q = queries(s, io, size=0.7)
+    flush = torch.empty(1 << 28, dtype=torch.uint8, device="cuda")
+    outs = []
+    for _ in range(4):
+        flush.zero_()
+        outs.append(s.kv.attend(0, q, s.batch, block_length=block))
+    s.kv.check()
+    assert all(torch.equal(o, outs[0]) for o in outs[1:])
+    verify_on_gpu(s, q, io, block, outs[0])
+
+
+def verify_on_gpu(s, q, io, block, out):
+    """Every row of the output against torch in float64."""
+    kv, group = s.kv_name, s.nh // s.nk
+    for i, (a, n) in enumerate(zip(s.q_lens, s.lens)):
+        k, v = gpu_values(s, "k", i, n), gpu_values(s, "v", i, n)
+        x = q[s.start[i]:s.start[i] + a].double().view(a, s.nk, group, s.d)
+        pos = torch.arange(n - a, n, device="cuda")
+        sees = torch.arange(n, device="cuda")[None, :] // block <= (pos // block)[:, None]
+        score = torch.einsum("ahgd,nhd->ahgn", x, k) * s.d ** -0.5
+        w = torch.softmax(score.masked_fill(~sees[:, None, None, :], -float("inf")), -1)
+        ref = torch.einsum("ahgn,nhd->ahgd", w, v)
+        size = torch.einsum("ahgn,nhd->ahgd", w, v.abs())
+        err = (out[s.start[i]:s.start[i] + a].double().view_as(ref) - ref).abs()
+        # as attend_tolerance: the weights' half step, the scores' errors (sums of d + 16 additions that may truncate, a
+        # query rounded to bf16 on bf16 pages) twice, the sums over the positions, the output's half step. The smallest
+        # step of f16 weights: 2^-25 of the largest weight times value scale, over n positions of at most 448 (e4m3)
+        bf = kv == "bf16"
+        dot = float(torch.einsum("ahgd,nhd->ahgn", x.abs(), k.abs()).max()) * s.d ** -0.5
+        ds = dot * ((s.d + 16) * 2.0 ** -23 + 2.0 ** -21 + (kv_ref.HALF_STEP["bf16"] if bf and io == "f16" else 0.0))
+        rel = kv_ref.HALF_STEP["bf16" if bf else "f16"] + 2 * np.expm1(ds + 2.0 ** -21) + (n / 8 + 64) * 2.0 ** -23
+        spread = 2.0 ** 6 if kv == "e4m3" else 1.0  # of the value scales
+        floor = 0.0 if bf else 2.0 ** -25 * float(w.max()) * n * float(v.abs().max()) * spread
+        tol = rel * size + kv_ref.HALF_STEP[io] * ref.abs() * 1.01 + floor + 2.0 ** -25
+        assert bool((err <= tol).all()), (i, float((err / tol).max()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv,heads_kv,dim", [("e4m3", 2, 128), ("bf16", 2, 64), ("f16", 4, 128)])
+def test_attend_many_unequal_sequences(kv, heads_kv, dim):
+    """Several items to a CTA, one after the other, of one and of two 128-row halves in any order."""
+    rng = np.random.default_rng(dim)
+    q_lens = rng.integers(1, 75, 170)
+    s = Setup(q_lens, rng.integers(0, 300, 170), kv, 16, heads_kv, dim, page=32, seed=7)
+    g = torch.Generator(device="cuda").manual_seed(2)
+    for held, scale in ((s.kv.k, s.kv.k_scale), (s.kv.v, s.kv.v_scale)):
+        held.copy_(torch.randn(held.shape, generator=g, device="cuda").to(held.dtype))
+        if kv == "e4m3":
+            scale.view(torch.uint8).copy_(torch.randint(121, 128, scale.shape, generator=g, device="cuda").to(torch.uint8))
+    q = queries(s, "bf16", size=0.7)
+    out = s.kv.attend(0, q, s.batch, block_length=1)
+    for _ in range(5):
+        assert torch.equal(s.kv.attend(0, q, s.batch, block_length=1), out)
+    s.kv.check()
+    verify_on_gpu(s, q, "bf16", 1, out)
+
+
 # ------------------------------------------------------------------------------------------------
 # append
 # ------------------------------------------------------------------------------------------------
