@@ -233,6 +233,13 @@ struct Walk {
   }
 };
 
+// 16 bytes that are used once: not kept in L1, whose data path the products' operands share
+__device__ __forceinline__ uint4 load_past_l1(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
 // mbar_wait by a whole warp, with one answer: after a timeout no lane goes on alone
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, uint32_t* err, uint32_t bit) {
   const bool ok = mbar_wait(bar, parity, err, bit);
@@ -961,12 +968,12 @@ __global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__
         if (!is_v && lt < 4 && tile * TILE + 32 * lt < lim) scale = p.pg.k_scale[scale_at] | p.pg.v_scale[scale_at] << 8;
         if ((tile + 1) * TILE <= lim) {
 #pragma unroll
-          for (int i = 0; i < N; ++i) x[i] = __ldg(reinterpret_cast<const uint4*>(source(i)));
+          for (int i = 0; i < N; ++i) x[i] = load_past_l1(source(i));
         } else {
 #pragma unroll
           for (int i = 0; i < N; ++i) {
             x[i] = make_uint4(0, 0, 0, 0);
-            if (tile * TILE + r0 + i * RPI < lim) x[i] = __ldg(reinterpret_cast<const uint4*>(source(i)));
+            if (tile * TILE + r0 + i * RPI < lim) x[i] = load_past_l1(source(i));
           }
         }
       }
