@@ -7,7 +7,8 @@
 // 32-bit angle is already 0.004 off); sine and cosine of its fraction in 32, with what the rounding left added.
 //
 // Pages of 8 bits: for each (32-position block, head) e = the smallest exponent with amax <= 448 * 2^e,
-// and e4m3(x * 2^-e) is stored. A power of two as scale loses nothing against any other scale (e4m3
+// and e4m3(x * 2^-e) is stored, as it follows from x in 64 bits (a 32-bit x turns a code in ten million, and a scale
+// now and then; keys are few beside the queries). A power of two as scale loses nothing against any other scale (e4m3
 // keeps 4 significant bits at every size) and makes the move of kept values to a new scale exact.
 //
 // Work unit: a 32-position block of one sequence that gains rows (the grid is an upper bound of their
@@ -17,10 +18,10 @@
 // until its amax is known. 16 lanes (head_dim 128) or 8 (64) share a row, 8 elements each: 16-byte
 // loads of 16-bit rows, two or four rows a warp at once, and half the shuffles of a warp per row.
 //
-// Measured on B200 (32 + 4 + 4 heads of 128, rotary_dim 64, e4m3): a 16384-token prompt, 318.8 MB, 101 us = 3.16 TB/s,
-// half the measured copy rate. Instruction issue is 71 % active there: norm, rotation and conversion take about 150
-// instructions per 8 elements, and that bounds it, not HBM. One block of 32 positions: 10 us a call, most of it the
-// launch and the host.
+// Measured on B200 (32 + 4 + 4 heads of 128, rotary_dim 64, e4m3): a 16384-token prompt, 318.8 MB, 118 us = 2.7 TB/s, 42 %
+// of the copy rate (101 us with keys in 32 bits). Instruction issue bounds it, not HBM: norm, rotation and conversion
+// take about 150 instructions per 8 elements. One block of 32 positions: 10 us a call, most of it the launch and
+// the host.
 #include <algorithm>
 #include <cmath>
 #include <cstdio>
@@ -36,6 +37,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxHalf = 64;  // rotary_dim / 2 at head_dim 128
+constexpr int kWantedHeld = 148 * 3;  // of them for the keys of 8-bit pages, whose table is dearer
 constexpr int kWanted = 148 * 6;  // CTAs of a large call (16384-token prompt: 125 us at 6 an SM, 134 at 12, 161 at 24)
 
 struct AppendParams {
@@ -182,6 +184,41 @@ __device__ __forceinline__ void norm_rotate(float (&x)[8], const float (&w)[8], 
   }
 }
 
+__device__ __forceinline__ double shfl_double(double x, int from) {
+  return __hiloint2double(__shfl_sync(0xffffffffu, __double2hiint(x), from), __shfl_sync(0xffffffffu, __double2loint(x), from));
+}
+
+// norm_rotate in 64 bits, for values that 3 bits are cut from next: each result is rounded to odd (cut to 32 bits, the
+// last bit set if anything was cut off), so that the second rounding, and the comparison with a scale's border,
+// come out as for the exact value.
+template <int LPR>
+__device__ __forceinline__ void norm_rotate_exact(float (&x)[8], const float (&w)[8], bool norm, float eps, int sub, int half,
+                                                  const double2* cs) {
+  double ss = 0.0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) ss = fma((double)x[i], (double)x[i], ss);
+#pragma unroll
+  for (int o = LPR / 2; o; o >>= 1) ss += shfl_double(ss, (threadIdx.x & 31) ^ o);
+  const double r = norm ? rsqrt(ss * (1.0 / (8 * LPR)) + (double)eps) : 1.0;
+  const int hl = half / 8;
+  const bool lo = sub < hl, in = sub < 2 * hl;
+  const int lane = threadIdx.x & 31, from = lane + (lo ? hl : in ? -hl : 0);
+  const double2* c = cs + 8 * (lo ? sub : in ? sub - hl : 0);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    double y = (double)x[i] * r * (double)w[i];
+    if (half) {
+      const double z = shfl_double(y, from);
+      if (in) {
+        const double2 t = c[i];
+        y = lo ? y * t.x - z * t.y : y * t.x + z * t.y;
+      }
+    }
+    const float f = __double2float_rz(y);
+    x[i] = (double)f == y ? f : __int_as_float(__float_as_int(f) | 1);
+  }
+}
+
 // Scale exponent of a block: amax = f 2^x with 1 <= f < 2, and 448 = 1.75 * 2^8.
 __device__ __forceinline__ int scale_exponent(float amax) {
   const uint32_t u = __float_as_uint(amax);
@@ -224,7 +261,10 @@ __global__ void __launch_bounds__(kThreads, 4) kv_append_kernel(const __grid_con
   constexpr int LPR = HD / 8;     // lanes a row
   constexpr int RPW = 32 / LPR;   // rows a warp holds at once
   constexpr int PASSES = kScaleBlock / (kWarps * RPW);
-  __shared__ __align__(16) float2 cs[kScaleBlock * kMaxHalf];
+  // (cos, sin) of the block's positions: [position][i] float2, or double2 for the keys of 8-bit pages
+  __shared__ __align__(16) uint8_t table[kScaleBlock * kMaxHalf * (KV == KV_E4M3 ? 16 : 8)];
+  float2* const cs = reinterpret_cast<float2*>(table);
+  double2* const cs64 = reinterpret_cast<double2*>(table);
   __shared__ float amax_s[2][kWarps];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, sub = lane % LPR;
 
@@ -281,6 +321,12 @@ __global__ void __launch_bounds__(kThreads, 4) kv_append_kernel(const __grid_con
     const int t = (int)((i * p.half_magic) >> 18), f = i - t * p.half;
     const double a = (double)(lo + t) * p.turns[f];
     const double turn = a - rint(a);
+    if (KV == KV_E4M3 && group >= p.flat_groups) {
+      double sn, c;
+      sincospi(2.0 * turn, &sn, &c);
+      cs64[(lo - b0 + t) * kMaxHalf + f] = make_double2(c, sn);
+      continue;
+    }
     const float hi = (float)turn, rest = 6.2831853f * (float)(turn - hi);  // what 24 bits leave of the angle
     float sn, c;
     sincospif(2.0f * hi, &sn, &c);
@@ -392,7 +438,7 @@ __global__ void __launch_bounds__(kThreads, 4) kv_append_kernel(const __grid_con
 #pragma unroll
         for (int i = 0; i < 8; ++i) y[i] = x[j][i];
         const bool now = b0 + t >= lo && b0 + t < hi;
-        norm_rotate<LPR>(y, wk, p.k_norm != nullptr, p.eps, sub, p.half, cs + (now ? t : lo - b0) * kMaxHalf);
+        norm_rotate_exact<LPR>(y, wk, p.k_norm != nullptr, p.eps, sub, p.half, cs64 + (now ? t : lo - b0) * kMaxHalf);
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[j][i] = now ? y[i] : x[j][i];
       }
@@ -533,13 +579,13 @@ extern "C" dmoe_status dmoe_kv_append(const dmoe_kv_cache* cache, const dmoe_kv_
   // Heads a CTA takes: as many as leave about kWanted CTAs (the rotation's table is then made for several heads; one
   // head each below that, where latency counts), but at least the 16 rows that the warps hold at once
   const int64_t fresh = std::max<int64_t>(1, std::min<int64_t>(kScaleBlock, a->n_tokens / std::max<int64_t>(1, units)));
-  auto share = [&](int64_t heads, int64_t least) {
-    const int64_t per = std::min<int64_t>(128, std::max((units * heads + kWanted - 1) / kWanted, least)), groups = (heads + per - 1) / per;
+  auto share = [&](int64_t heads, int64_t least, int64_t wanted) {
+    const int64_t per = std::min<int64_t>(128, std::max((units * heads + wanted - 1) / wanted, least)), groups = (heads + per - 1) / per;
     return (int)((heads + groups - 1) / groups);  // even groups
   };
-  p.flat_per_cta = share(p.flat_slots, std::min<int64_t>(p.flat_slots, (16 + fresh - 1) / fresh));
+  p.flat_per_cta = share(p.flat_slots, std::min<int64_t>(p.flat_slots, (16 + fresh - 1) / fresh), kWanted);
   p.flat_groups = (p.flat_slots + p.flat_per_cta - 1) / p.flat_per_cta;
-  p.held_per_cta = held ? share(nk, 1) : 1;
+  p.held_per_cta = held ? share(nk, 1, kWantedHeld) : 1;
   p.held_groups = held ? (nk + p.held_per_cta - 1) / p.held_per_cta : 0;
   const dim3 grid((unsigned)units, (unsigned)(p.flat_groups + 2 * p.held_groups));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
