@@ -322,6 +322,8 @@ def verify_on_gpu(s, q, io, block, out):
     """Every row of the output against torch in float64."""
     kv, group = s.kv_name, s.nh // s.nk
     for i, (a, n) in enumerate(zip(s.q_lens, s.lens)):
+        if a == 0:
+            continue
         k, v = gpu_values(s, "k", i, n), gpu_values(s, "v", i, n)
         x = q[s.start[i]:s.start[i] + a].double().view(a, s.nk, group, s.d)
         pos = torch.arange(n - a, n, device="cuda")
@@ -575,3 +577,45 @@ def test_append_then_attend(kv, q):
         _, rot = append_and_check(s, "f32", "bf16", batch=batch, lens=lens)
         check_attend(s, rot, "bf16", 32 if q == 32 else 1, batch=batch, lens=lens, rows=8)
         at = [at[0] + q, at[1] + (q if step % 2 else 0)]  # sequence 1 writes some blocks twice
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv", ["e4m3", "bf16"])
+def test_offsets_past_32_bits(kv):
+    """Pages whose bytes, elements and rows lie past 2^32: the same results as on the first pages."""
+    n_pages = 40000 if kv == "e4m3" else 34000  # 8 heads x 128 positions x 128: 5.2 GB of bytes, 4.4 G elements
+    cache = dm.PagedKV(n_pages=n_pages, n_head_kv=8, head_dim=128, page_size=128, kv_type=kv)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    for rows, n_head in ((1, 8), (200, 16)):
+        qkv = torch.randn(rows, (n_head + 16) * 128, generator=g, device="cuda")
+        got = []
+        for pages in ([0, 1], [n_pages - 1, n_pages - 2]):
+            batch = cache.batch(i32([pages]), i32([0, rows]), i32([rows + 7]), rows)
+            for p in pages:  # the seven positions before
+                cache.k[0, p].view(torch.uint8).zero_(), cache.v[0, p].view(torch.uint8).zero_()
+                if kv == "e4m3":
+                    cache.k_scale.view(torch.uint8)[0, p] = 127
+                    cache.v_scale.view(torch.uint8)[0, p] = 127
+            q = cache.append(0, qkv, batch, n_head=n_head, rotary_dim=64, q_type=torch.bfloat16)
+            got.append((q, cache.k[0, pages].view(torch.uint8).clone(), cache.v[0, pages].view(torch.uint8).clone(),
+                        cache.attend(0, q, batch)))
+        cache.check()
+        assert all(torch.equal(a, b) for a, b in zip(*got))
+        assert bool(got[0][1].any()) and bool((got[0][3] != 0).any())
+
+
+@pytest.mark.gpu
+def test_thousands_of_sequences():
+    """More sequences than a CTA has threads, most of them of one row."""
+    rng = np.random.default_rng(5)
+    q_lens = np.where(rng.random(3000) < 0.02, 20, 1) * (rng.random(3000) < 0.9)
+    s = Setup(q_lens, rng.integers(0, 40, 3000), "e4m3", 4, 2, 64, page=32, seed=11, fill=False)
+    g = torch.Generator(device="cuda").manual_seed(2)
+    for held, scale in ((s.kv.k, s.kv.k_scale), (s.kv.v, s.kv.v_scale)):
+        held.copy_(torch.randn(held.shape, generator=g, device="cuda").to(held.dtype))
+        scale.view(torch.uint8).fill_(126)
+    _, rot = append_and_check(s, "f32", "bf16", rot=32)
+    out = s.kv.attend(0, rot, s.batch)
+    s.kv.check()
+    verify_on_gpu(s, rot, "bf16", 1, out)
