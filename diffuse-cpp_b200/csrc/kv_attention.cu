@@ -748,8 +748,8 @@ __global__ void __launch_bounds__(32 * RowsCfg<HD, KV, NT>::kWarps, 1) kv_rows_k
 // Many rows (denoising blocks, prompts): tensor-core tiles of 2 x 128 rows by 128 positions.
 //
 // One persistent CTA per SM. Warps 0-3 and 4-7: softmax of the two 128-row halves, a thread a row; warps
-// 8-11: keys and values from the pages into shared memory, as 16-bit operands in the 128-byte swizzle;
-// warp 12 issues the products. TMEM: two score tiles (f32, 128 columns each; a half's weights
+// 8-11: keys, 12-15: values, from the pages into shared memory as 16-bit operands in the 128-byte swizzle; a
+// thread of warp 16 issues the products. TMEM: two score tiles (f32, 128 columns each; a half's weights
 // overwrite its scores as the 16-bit A operand of the second product) and two outputs. The products of one
 // half run while the other half's softmax does. The running maximum that weights refer to follows
 // the true one only when that is 2^8 ahead (f16 holds the weights up to then), so an output is
