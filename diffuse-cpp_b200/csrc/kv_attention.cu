@@ -32,6 +32,8 @@ namespace dmoe {
 namespace {
 
 constexpr int kMaxGrid = 148;  // one CTA an SM
+// The least factor of a score. Operands are at most 1 (queries) and 65504, so below it no score counts
+constexpr float kTinyFactor = 0x1p-126f;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 // An item that a CTA begins and does not end
@@ -1146,7 +1148,7 @@ __global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__
             const float amax = p.is_bf16 ? __uint_as_float(a << 16) : __half2float(__ushort_as_half((uint16_t)a));
             const int e = min(max((int)(__float_as_uint(amax) >> 23) - 126, -100), 100);
             inv = pow2i(-e);
-            factor *= pow2i(e);
+            factor = fmaxf(factor * pow2i(e), kTinyFactor);
           }
 #pragma unroll 2
           for (int i = 0; i < HD / 8; ++i) {
@@ -1204,7 +1206,9 @@ __global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__
         if (KV == KV_E4M3) {
           const float4 k = *reinterpret_cast<const float4*>(scale_s[0][n & 3]), v = *reinterpret_cast<const float4*>(scale_s[1][n & 3]),
                        u = *reinterpret_cast<const float4*>(scale_s[2][n & 3]);
-          c[0] = factor * k.x, c[1] = factor * k.y, c[2] = factor * k.z, c[3] = factor * k.w;
+          // not down to zero (tiny queries over zero keys): masked scores are -inf when they are multiplied
+          c[0] = fmaxf(factor * k.x, kTinyFactor), c[1] = fmaxf(factor * k.y, kTinyFactor);
+          c[2] = fmaxf(factor * k.z, kTinyFactor), c[3] = fmaxf(factor * k.w, kTinyFactor);
           ev[0] = v.x, ev[1] = v.y, ev[2] = v.z, ev[3] = v.w;
           un[0] = u.x, un[1] = u.y, un[2] = u.z, un[3] = u.w;
         } else {
