@@ -10,8 +10,10 @@
 // for every 32 positions; e4m3 is exact in f16, so the products run in f16 on the codes:
 //   t_j = log2(e) scale 2^ek (q.kc_j) + ev,  M = max t_j,  p_j = 2^(t_j - M),
 //   o = sum p_j vc_j / sum p_j 2^-ev.
-// The value scale rides in the exponent, so p <= 1 is rounded to f16 relative to the largest weight
-// times value scale and neither factor can leave f16's range. Queries are brought into [-1, 1] by a
+// The value scale rides in the exponent, so p is rounded to f16 relative to the largest weight times value
+// scale. f16 has 30 binades of whole precision: M is held below the true maximum (kLift), so that the largest
+// weights are near f16's top and those of positions beside one that takes nearly all the weight (an attention
+// sink, whose value is often next to zero) are not rounded to a few bits. Queries are brought into [-1, 1] by a
 // power of two per row (exact). M and both sums are 32-bit; p is rounded once, to the products' type.
 //
 // Work split: the tiles of all (sequence, row tile, key/value head) items are numbered through, and every
@@ -41,6 +43,14 @@ struct Spanning {
   int last;  // CTA that ends it; -1: there is none
   int row0, row_lo, rows, head;  // the sequence's first row, the item's rows [row_lo, row_lo + rows) of q_len * group
   int pad[3];
+};
+
+// Weights of f16 products are 2^kLift times what they are of the maximum's: up to 2^15. The tiles let them grow to that
+// before their reference follows the maximum, so it begins 2^8 lower. bf16 has the range as it is.
+template <int KV>
+struct Lift {
+  static constexpr float kRows = KV == KV_BF16 ? 0.f : 15.f;
+  static constexpr float kTiles = KV == KV_BF16 ? 0.f : 7.f, kGrown = kTiles + 8.f;
 };
 
 struct AttnParams {
@@ -572,7 +582,7 @@ __global__ void __launch_bounds__(32 * RowsCfg<HD, KV, NT>::kWarps, 1) kv_rows_k
         for (int i = 0; i < 2; ++i) {
 #pragma unroll
           for (int off = 4; off < 32; off <<= 1) mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], off));
-          const float mn = fmaxf(m[n][i], mx[i]);
+          const float mn = fmaxf(m[n][i], __fsub_ru(mx[i], Lift<KV>::kRows));  // no weight is past 2^15, however large mx
           base[i] = mn == -INFINITY ? 0.f : mn;
           shrink[i] = ex2(m[n][i] - base[i]);
           m[n][i] = mn;
@@ -753,9 +763,9 @@ __global__ void __launch_bounds__(32 * RowsCfg<HD, KV, NT>::kWarps, 1) kv_rows_k
 // 8-11: keys, 12-15: values, from the pages into shared memory as 16-bit operands in the 128-byte swizzle; a
 // thread of warp 16 issues the products. TMEM: two score tiles (f32, 128 columns each; a half's weights
 // overwrite its scores as the 16-bit A operand of the second product) and two outputs. The products of one
-// half run while the other half's softmax does. The running maximum that weights refer to follows
-// the true one only when that is 2^8 ahead (f16 holds the weights up to then), so an output is
-// rescaled in TMEM only then.
+// half run while the other half's softmax does. The reference of a row's weights (Lift) follows
+// the running maximum only when that is 2^8 ahead of where it was set, so an output is rescaled in TMEM only
+// then.
 // Bound by a half's chain of scores (512 cycles of the tensor pipe), exponentials (128 a thread, 8 cycles a warp:
 // 1024 at least) and products (512), of which two are in flight: about 3800 cycles for two tiles. Measured: 2048 rows
 // over 16384 positions of bf16 pages 530 us = 0.98 PFLOP/s (tensor pipe 55 % active, exponential unit 55 %); 16
@@ -1249,8 +1259,8 @@ __global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__
           mx = m;
         }
         float shrink = 1.f;
-        if (mx > m + 8.f || m == -INFINITY) {
-          const float to = fmaxf(m, mx);
+        if (mx - m > Lift<KV>::kGrown || m == -INFINITY) {
+          const float to = fmaxf(m, __fsub_ru(mx, Lift<KV>::kTiles));
           shrink = to == -INFINITY ? 1.f : ex2(m - to);
           m = to;
           l *= shrink;
