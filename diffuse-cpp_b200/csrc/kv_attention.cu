@@ -1259,8 +1259,10 @@ __global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__
           mx = m;
         }
         float shrink = 1.f;
-        if (mx - m > Lift<KV>::kGrown || m == -INFINITY) {
-          const float to = fmaxf(m, __fsub_ru(mx, Lift<KV>::kTiles));
+        // at least the largest score as the weights' fma has it, exact: mx was rounded, by far more than 1 where it is huge
+        const float most = fmaf(fabsf(mx), 0x1p-23f, mx);
+        if (most - m > Lift<KV>::kGrown || m == -INFINITY) {
+          const float to = fmaxf(m, __fsub_ru(most, Lift<KV>::kTiles));
           shrink = to == -INFINITY ? 1.f : ex2(m - to);
           m = to;
           l *= shrink;
