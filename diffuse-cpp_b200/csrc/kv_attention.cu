@@ -803,7 +803,8 @@ __global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__
   __shared__ uint32_t tmem_base_s;
   __shared__ int sums[C::kThreads / 32];
   __shared__ Run found;
-  __shared__ int not_finite_from[4][HD];  // [item of the run & 3][d]: first position whose value is not finite
+  // [item of the run & 3][sign][d]: first position whose value is +inf, or -inf; both for NaN
+  __shared__ int not_finite_from[4][2][HD];
   __shared__ int any_not_finite[4];
   // scales of keys, exponents of values and their reciprocal scales [..][tile of the run & 3][32-position block].
   // Written with the keys, before their arrival; the slot is free again when the tile two on has been multiplied by
@@ -962,14 +963,15 @@ __global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__
     auto source = [&](int i) { return block_at[i * RPI / 32] + (i * RPI % 32) * (HD * ES); };
     // Values at positions that only some rows see, where they are not finite: their products with a zero
     // weight would reach the other rows. They are set to zero, and their element marked for the rows that see them
-    auto mark = [&](int seg, int pos, int d) {
-      atomicMin(&not_finite_from[seg & 3][d], pos);
+    auto mark = [&](int seg, int pos, int d, bool plus, bool minus) {
+      if (plus) atomicMin(&not_finite_from[seg & 3][0][d], pos);
+      if (minus) atomicMin(&not_finite_from[seg & 3][1][d], pos);
       any_not_finite[seg & 3] = 1;
     };
     auto reset_marks = [&](int seg) {
       // once both halves have read the buffer's last use, four items back
       if (!warp_wait(&bar.read[seg & 3], ((seg >> 2) & 1) ^ 1, err, kTimeout)) return false;
-      if (lt < HD) not_finite_from[seg & 3][lt] = INT32_MAX;
+      if (lt < HD) not_finite_from[seg & 3][0][lt] = not_finite_from[seg & 3][1][lt] = INT32_MAX;
       if (lt == 0) any_not_finite[seg & 3] = 0;
       mbar_arrive(&bar.reset);
       return warp_wait(&bar.reset, seg & 1, err, kTimeout);
@@ -1025,7 +1027,7 @@ __global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__
                 const uint32_t bad = __vcmpeq4(v[e] & 0x7f7f7f7fu, 0x7f7f7f7fu);
                 if (bad && pos >= lim_min) {
                   for (int b = 0; b < 4; ++b)
-                    if ((bad >> (8 * b)) & 1u) mark(seg, pos, 16 * c + 4 * e + b);
+                    if ((bad >> (8 * b)) & 1u) mark(seg, pos, 16 * c + 4 * e + b, true, true);
                   v[e] &= ~bad;
                 }
               }
@@ -1078,8 +1080,12 @@ __global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__
                 constexpr uint32_t kExp = kBf ? 0x7f807f80u : 0x7c007c00u;
                 const uint32_t bad = __vcmpeq2(v[e] & kExp, kExp);
                 if (bad && pos >= lim_min) {
-                  for (int b = 0; b < 2; ++b)
-                    if ((bad >> (16 * b)) & 1u) mark(seg, pos, 8 * c + 2 * e + b);
+                  for (int b = 0; b < 2; ++b) {
+                    if (!((bad >> (16 * b)) & 1u)) continue;
+                    const uint32_t h = v[e] >> (16 * b) & 0xffffu;
+                    const bool nan = (h & ~kExp & 0x7fffu) != 0;
+                    mark(seg, pos, 8 * c + 2 * e + b, nan || !(h & 0x8000u), nan || (h & 0x8000u));
+                  }
                   v[e] &= ~bad;
                   any = true;
                 }
@@ -1345,11 +1351,14 @@ __global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__
         tmem_wait_ld();
         if (marked) {
 #pragma unroll 1
-          for (int i = 0; i < 32; ++i)
-            if (*const_cast<volatile int*>(&not_finite_from[seg & 3][d0 + i]) < lim) {
+          for (int i = 0; i < 32; ++i) {
+            const float plus = *const_cast<volatile int*>(&not_finite_from[seg & 3][0][d0 + i]) < lim ? INFINITY : 0.f;
+            const float minus = *const_cast<volatile int*>(&not_finite_from[seg & 3][1][d0 + i]) < lim ? INFINITY : 0.f;
+            if (plus + minus != 0.f) {
 #pragma unroll
-              for (int e = 0; e < 32; ++e) x[e] = e == i ? 0x7fc00000u : x[e];
+              for (int e = 0; e < 32; ++e) x[e] = e == i ? __float_as_uint(__uint_as_float(x[e]) + (plus - minus)) : x[e];
             }
+          }
         }
         if (!whole) {
           if (live) {

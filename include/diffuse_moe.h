@@ -377,7 +377,8 @@ dmoe_status dmoe_kv_append(const dmoe_kv_cache* cache, const dmoe_kv_batch* batc
  * logarithm of each softmax's sum, -inf for rows that see nothing (their output is zero). q and out:
  * DMOE_TYPE_F16 or BF16, of one type; rows of q_stride / out_stride elements. workspace: DEVICE,
  * 16-byte aligned, dmoe_kv_attention_workspace() bytes, uninitialised; calls that may overlap need one
- * each. A value that is not finite reaches only the rows that see its position.
+ * each. A value that is not finite reaches only the rows that see its position (an infinity as one,
+ * unless its weight rounds to zero).
  * Products are rounded once, to f16 (e4m3 and f16 pages) or bf16 (bf16 pages, where f16 queries are
  * rounded to bf16 first); maxima, sums and outputs are 32-bit until the output's own rounding. */
 typedef struct dmoe_kv_attention_args {
