@@ -708,6 +708,9 @@ class PagedKV:
     def check(self) -> None:
         """Waits for the device and raises if a kernel met a page number or a batch entry out of its bounds
         since the last check (such entries are skipped, see include/diffuse_moe.h)."""
+        import torch
+
+        torch.cuda.synchronize(self.device)  # calls on every stream, not the current one alone
         bits = int(self.err.item())
         if bits:
             self.err.zero_()
