@@ -377,7 +377,8 @@ def generate_batch(model: LLaDA2Model, prompts: list, n_generate: int, steps: in
     each sequence that is not done, whatever their lengths and positions. Sequence i generates blocks until
     n_generate positions past its prompt are covered, as generate() does. Returns the sequences (int32 numpy)
     and the number of forwards. kv: a cache from model.new_paged() to use (its pages are taken from the first
-    on; default: a new one of kv_type). sampler: as for generate()."""
+    on; default: a new one of kv_type). sampler: as for generate(). Raises DmoeError for what the cache's kernels
+    report (kv.check())."""
     sample = dm.sample_step if sampler is None else sampler
     c, dev = model.cfg, model.device
     L = c.block_length
@@ -435,7 +436,10 @@ def generate_batch(model: LLaDA2Model, prompts: list, n_generate: int, steps: in
     token = torch.empty((len(prompts), L), dtype=torch.int32, device=dev)
     prob = torch.empty((len(prompts), L), dtype=torch.float32, device=dev)
     ncom = torch.zeros(len(prompts), dtype=torch.int32, device=dev)
+    report = getattr(kv, "check", None)  # a stand-in without kernels has no error word
     while True:
+        if report is not None:
+            report()  # attention that is not complete, or that read wrong pages, ends the generation
         live = [i for i in range(len(prompts)) if blk[i] < n_blocks[i] and step[i] < len(sched)]
         if not live:
             return [s.cpu().numpy() for s in seqs], forwards
