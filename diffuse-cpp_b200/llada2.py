@@ -237,11 +237,13 @@ class LLaDA2Model:
                           kv_type=kv_type, n_layer=c.n_layer, device=self.device)
 
     def forward_paged(self, tokens: torch.Tensor, kv: dm.PagedKV, batch: dm.KVBatch,
-                      stream: Optional[int] = None) -> torch.Tensor:
+                      stream: Optional[int] = None, rows: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Logits [n, n_vocab] f32 of the batch's rows: `tokens` (int64 [n]) holds each sequence's last positions,
         whole blocks of them, one sequence after the other (kv.batch(...)). Their keys and values are written into
         the pages; each row attends to its sequence's positions up to the end of its own block. The same
-        as forward() of each sequence over its own cache, up to the pages' rounding."""
+        as forward() of each sequence over its own cache, up to the pages' rounding. rows (int64 indices, any number):
+        the logits of these rows alone, in their order (a prefill reads none, and all of them are 6 bytes a row and
+        vocabulary entry)."""
         c = self.cfg
         n = int(tokens.shape[0])
         if n > self._max_n:
@@ -268,6 +270,10 @@ class LLaDA2Model:
             else:
                 self.moe[il].forward(h.contiguous(), out=y, stream=stream)
                 x = y + residual
+        if rows is not None:
+            if rows.numel() == 0:
+                return x.new_empty((0, c.n_vocab))
+            x = x[rows]
         return self._lin(rms_norm(x, self.w["output_norm"], c.rms_eps), "output")
 
 
@@ -371,6 +377,10 @@ def generate(model: LLaDA2Model, prompt: np.ndarray, n_generate: int, steps: int
     return seq.cpu().numpy(), forwards
 
 
+#: Rows of one prefill call of generate_batch: the activations of a call grow with them.
+PREFILL_ROWS = 16384
+
+
 def generate_batch(model: LLaDA2Model, prompts: list, n_generate: int, steps: int = 8, threshold: float = 0.95,
                    kv_type: str = "e4m3", page_size: int = 64, kv=None, sampler=None) -> tuple:
     """generate() for several prompts at once over one paged cache: every forward takes one denoising step of
@@ -403,22 +413,37 @@ def generate_batch(model: LLaDA2Model, prompts: list, n_generate: int, steps: in
         s[: len(p)] = torch.as_tensor(p, dtype=torch.int32, device=dev)
         seqs.append(s)
 
-    def forward(which: list, rows: list) -> torch.Tensor:
-        """The logits of rows (begin, end) of each of the sequences `which`, one after the other."""
+    def forward(which: list, rows: list, last: int) -> torch.Tensor:
+        """Rows (begin, end) of each of the sequences `which`, one after the other; the logits of the `last` last
+        ones of each."""
         lens = [e - b for b, e in rows]
+        ends = np.cumsum(lens)
         i32 = lambda v: torch.tensor(v, dtype=torch.int32).to(dev)  # noqa: E731
-        batch = kv.batch(tables[torch.tensor(which, device=dev)], i32([0] + list(np.cumsum(lens))),
-                         i32([e for _, e in rows]), max(lens))
-        return model.forward_paged(torch.cat([seqs[i][b:e] for i, (b, e) in zip(which, rows)]).long(), kv, batch)
+        batch = kv.batch(tables[torch.tensor(which, device=dev)], i32([0] + list(ends)), i32([e for _, e in rows]), max(lens))
+        wanted = None  # all of them
+        if lens != [last] * len(lens):
+            wanted = torch.from_numpy((ends[:, None] + np.arange(-last, 0)).ravel()).to(dev)
+        return model.forward_paged(torch.cat([seqs[i][b:e] for i, (b, e) in zip(which, rows)]).long(), kv, batch, rows=wanted)
 
-    # every whole prompt block but the last enters the cache at once
+    # every whole prompt block but the last enters the cache first, PREFILL_ROWS rows (whole blocks) a call
     blk = [len(p) // L for p in prompts]
     final = [max(0, b - 1) * L for b in blk]  # positions whose keys and values are final
     forwards = 0
-    first = [i for i, f in enumerate(final) if f > 0]
-    if first:
-        forward(first, [(0, final[i]) for i in first])
-        forwards += 1
+    some = max(1, PREFILL_ROWS // L) * L
+    calls = [[]]  # of (sequence, first row, last row + 1)
+    for i, f in enumerate(final):
+        b = 0
+        while b < f:
+            room = some - sum(y - x for _, x, y in calls[-1])
+            if room == 0:
+                calls.append([])
+                continue
+            calls[-1].append((i, b, min(f, b + room)))
+            b = calls[-1][-1][2]
+    for call in calls:
+        if call:
+            forward([i for i, _, _ in call], [(b, e) for _, b, e in call], 0)
+            forwards += 1
     step = [0] * len(prompts)
     left = [0] * len(prompts)
 
@@ -444,12 +469,10 @@ def generate_batch(model: LLaDA2Model, prompts: list, n_generate: int, steps: in
         if not live:
             return [s.cpu().numpy() for s in seqs], forwards
         rows = [(final[i], (blk[i] + 1) * L) for i in live]  # the previous block, where it is new, and this one
-        logits = forward(live, rows)
+        logits = forward(live, rows, L)
         forwards += 1
-        end = 0
-        for i, (b, e) in zip(live, rows):
-            end += e - b
-            sample(logits[end - L: end].contiguous(), seqs[i][e - L: e], c.mask_token_id, sched[step[i]], threshold,
+        for at, (i, (_, e)) in enumerate(zip(live, rows)):
+            sample(logits[at * L: (at + 1) * L].contiguous(), seqs[i][e - L: e], c.mask_token_id, sched[step[i]], threshold,
                    token[i], prob[i], ncom[i: i + 1])
         done = ncom.tolist()
         for i, (_, e) in zip(live, rows):
