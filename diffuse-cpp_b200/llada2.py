@@ -243,7 +243,11 @@ class LLaDA2Model:
         the pages; each row attends to its sequence's positions up to the end of its own block. The same
         as forward() of each sequence over its own cache, up to the pages' rounding. rows (int64 indices, any number):
         the logits of these rows alone, in their order (a prefill reads none, and all of them are 6 bytes a row and
-        vocabulary entry)."""
+        vocabulary entry). stream: the raw CUDA stream that the whole forward runs on (default: the current one); the
+        inputs must be ready there."""
+        if stream is not None:
+            with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=self.device)):
+                return self.forward_paged(tokens, kv, batch, rows=rows)
         c = self.cfg
         n = int(tokens.shape[0])
         if n > self._max_n:
