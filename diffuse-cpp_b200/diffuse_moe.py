@@ -710,7 +710,8 @@ class PagedKV:
         since the last check (such entries are skipped, see include/diffuse_moe.h)."""
         import torch
 
-        torch.cuda.synchronize(self.device)  # calls on every stream, not the current one alone
+        if self.err.is_cuda:
+            torch.cuda.synchronize(self.device)  # calls on every stream, not the current one alone
         bits = int(self.err.item())
         if bits:
             self.err.zero_()
