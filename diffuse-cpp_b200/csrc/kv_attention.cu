@@ -136,7 +136,8 @@ __device__ __forceinline__ Item item_of(const AttnParams& p, int u) {
 
 // Beginning and ending an item costs about as much as OV tiles. An item of t tiles is OV + t units long, and
 // the units of all items are numbered through; its tiles are the last t. With p.whole an item is one unit.
-// The host refuses calls whose units could number 2^31 or more.
+// The host refuses calls whose units could number 2^31 or more; sequences that overlap (a broken q_start) could still
+// have more, which find_run reports.
 struct Run {   // a CTA's run of units
   Item it;     // first item
   int u, head;
@@ -146,37 +147,41 @@ struct Run {   // a CTA's run of units
   int first;   // number of the first unit
 };
 
-// The whole CTA: finds its run. sums: THREADS / 32 words of shared memory.
+// The whole CTA: finds its run. sums: THREADS / 32 elements of shared memory.
 template <int R, int TILE, int OV, int THREADS>
-__device__ __forceinline__ Run find_run(const AttnParams& p, int* sums, Run* found) {
+__device__ __forceinline__ Run find_run(const AttnParams& p, int64_t* sums, Run* found) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int n_u = p.b.n_seq * p.n_qt;
   const int per = (n_u + THREADS - 1) / THREADS;
   const int u0 = min((int64_t)n_u, (int64_t)per * tid), u1 = min((int64_t)n_u, (int64_t)u0 + per);
-  int mine = 0;
+  int64_t incl = 0, mine;
   for (int u = u0; u < u1; ++u) {
     const int t = item_of<R, TILE>(p, u).tiles;
-    if (t) mine += p.whole ? 1 : t + OV;
+    if (t) incl += p.whole ? 1 : t + OV;
   }
-  int incl = mine;
+  mine = incl;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, incl, o);
+    const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += v;
   }
   if (lane == 31) sums[warp] = incl;
   if (tid == 0) found->left = 0;
   __syncthreads();
-  int before = incl - mine, total = 0;
+  int64_t before = incl - mine, all = 0;
   for (int w = 0; w < THREADS / 32; ++w) {
     if (w < warp) before += sums[w];
-    total += sums[w];
+    all += sums[w];
   }
   const int heads = p.pg.n_head_kv;
-  total *= heads;
+  if (all * heads > INT32_MAX) {  // the whole grid alike: no runs
+    if (tid == 0) kv_report(p.pg.err, DMOE_KV_ERR_BATCH);
+    all = 0;
+  }
+  const int total = (int)(all * heads);
   const int chunk = (int)(((uint32_t)total + gridDim.x - 1) / gridDim.x);
   const int first = (int)min((int64_t)chunk * blockIdx.x, (int64_t)total);
-  before *= heads;
+  before *= heads;  // in range wherever there is a run
   if (first < total && first >= before && first < before + mine * heads) {
     for (int u = u0; u < u1; ++u) {
       const Item it = item_of<R, TILE>(p, u);
@@ -184,8 +189,8 @@ __device__ __forceinline__ Run find_run(const AttnParams& p, int* sums, Run* fou
       if (first < before + w * heads) {
         found->it = it;
         found->u = u;
-        found->head = (first - before) / w;
-        found->unit = (first - before) % w;
+        found->head = (int)(first - before) / w;
+        found->unit = (int)(first - before) % w;
         found->left = min(chunk, total - first);
         break;
       }
@@ -402,7 +407,7 @@ __global__ void __launch_bounds__(32 * RowsCfg<HD, KV, NT>::kWarps, 1) kv_rows_k
   constexpr int VW = VB / 4;
   constexpr int JT = HD / 16;              // 16-row tiles of o^T
   extern __shared__ __align__(128) float smem_f[];
-  __shared__ int sums[C::kWarps];
+  __shared__ int64_t sums[C::kWarps];
   __shared__ Run found;
   __shared__ uint64_t bar[C::kWarps][C::kStages];  // a stage's copies have arrived
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
@@ -801,7 +806,7 @@ __global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__
   extern __shared__ uint8_t smem_raw[];
   __shared__ TileBars bar;
   __shared__ uint32_t tmem_base_s;
-  __shared__ int sums[C::kThreads / 32];
+  __shared__ int64_t sums[C::kThreads / 32];
   __shared__ Run found;
   // [item of the run & 3][sign][d]: first position whose value is +inf, or -inf; both for NaN
   __shared__ int not_finite_from[4][2][HD];
@@ -1690,10 +1695,10 @@ extern "C" dmoe_status dmoe_kv_attention(const dmoe_kv_cache* cache, const dmoe_
   if (((int64_t)std::min<int64_t>(batch->max_q_len, a->n_tokens) * group + 7) * std::max(1, batch->n_seq) > INT32_MAX)
     return fail(DMOE_ERR_UNSUPPORTED, "n_seq * max_q_len * n_head / n_head_kv must be below 2^31");
   {
-    // units of work, at most: row tiles of 8 or 256 rows, by tiles of 128 positions at least
+    // units of work, at most: row tiles of 8 or 256 rows, by tiles of 128 positions at least (the last one partly filled)
     const int64_t rows = max_rows_of(cache, batch, a), tile = rows <= kRowsMax ? 8 : 256;
     const double items = std::min((double)batch->n_seq * ((rows + tile - 1) / tile), (double)a->n_tokens * group / tile + batch->n_seq);
-    if (items * ((double)batch->max_pages * cache->page_size / 128 + 4) * cache->n_head_kv >= 2147483648.0)
+    if (items * (std::ceil((double)batch->max_pages * cache->page_size / 128) + 4) * cache->n_head_kv >= 2147483648.0)
       return fail(DMOE_ERR_UNSUPPORTED, "rows times positions of the page table too many for one call");
   }
   if (a->n_tokens == 0 || batch->n_seq == 0 || batch->max_q_len == 0) return DMOE_OK;

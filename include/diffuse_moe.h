@@ -326,7 +326,8 @@ typedef struct dmoe_kv_cache {
                                   attention then reads page 0 in its place */
 #define DMOE_KV_ERR_BATCH 2u   /* q_start not ascending within [0, n_tokens], kv_len negative or over
                                   max_pages pages, or more than max_q_len queries: the sequence is
-                                  skipped (its rows are left as they were) */
+                                  skipped (its rows are left as they were); or sequences that overlap so
+                                  far that an attention's work passes 2^31 units: nothing is computed */
 #define DMOE_KV_ERR_TIMEOUT 4u /* a bounded device-side wait expired: the outputs are not complete */
 
 /* The sequences of a call. Sequence s owns the rows [q_start[s], q_start[s + 1]) of the row tensors;
