@@ -339,12 +339,14 @@ __global__ void __launch_bounds__(kThreads, 4) kv_append_kernel(const __grid_con
     if (rel == 0 && pos0 < 0) {  // padding rows: zero queries
       const int pad = min(-pos0, q.q_len);
       const float zero[8] = {};
-      for (int r = tid; r < pad * nh * LPR; r += kThreads) {
-        const int h = h0 + (r / LPR) % nh;
-        if (h < p.n_head)
-          store8(p.q_out, (int64_t)(q.row0 + r / LPR / nh) * p.q_stride + (int64_t)h * HD + 8 * (r % LPR), p.q_type,
-                 p.vec_out, zero);
-      }
+      constexpr int kSome = 1 << 16;  // rows at a time, so that 8-element pieces are numbered in 31 bits
+      for (int first = 0; first < pad; first += min(kSome, pad - first))
+        for (int r = tid; r < min(kSome, pad - first) * nh * LPR; r += kThreads) {
+          const int h = h0 + (r / LPR) % nh;
+          if (h < p.n_head)
+            store8(p.q_out, (int64_t)(q.row0 + first + r / LPR / nh) * p.q_stride + (int64_t)h * HD + 8 * (r % LPR), p.q_type,
+                   p.vec_out, zero);
+        }
     }
     float wq[8], wk[8];
     load_weights(p.q_norm, sub, wq);
