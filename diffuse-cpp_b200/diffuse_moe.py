@@ -576,7 +576,7 @@ class PagedKV:
     positions, shared by every sequence of a batch. kv_type "bf16", "f16", or "e4m3": 8 bits with a
     power-of-two scale for every 32 positions of a head. k and v are [n_layer, n_pages, n_head_kv,
     page_size, head_dim] (zeroed); in 8-bit pages k_scale and v_scale [n_layer, n_pages, n_head_kv,
-    page_size / 32] are torch.float8_e8m0fnu, and a value is code * scale.
+    page_size / 32] are torch.float8_e8m0fnu (at first the smallest, 2^-60), and a value is code * scale.
 
     append() writes a layer's new keys and values and returns the rotated queries; attend() is the
     attention of queries over the pages. Both enqueue on the current torch stream (or `stream`) and can
@@ -598,7 +598,8 @@ class PagedKV:
                           for _ in range(2))
         self.k_scale = self.v_scale = None
         if kv_type == "e4m3":
-            self.k_scale, self.v_scale = (torch.zeros(*shape[:3], max(1, page_size // 32), dtype=torch.uint8, device=device)
+            # byte 67: 2^-60, the scale of a block of zeros
+            self.k_scale, self.v_scale = (torch.full((*shape[:3], max(1, page_size // 32)), 67, dtype=torch.uint8, device=device)
                                           .view(torch.float8_e8m0fnu) for _ in range(2))
         self.err = torch.zeros(1, dtype=torch.int32, device=device)
         self.device = self.err.device
