@@ -158,13 +158,21 @@ __device__ __forceinline__ void norm_rotate(float (&x)[8], const float (&w)[8], 
   for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
 #pragma unroll
   for (int o = LPR / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  float r = 1.0f;
-  if (norm) {
-    const float m = fmaf(ss, 1.0f / (8 * LPR), eps);
+  float m = fmaf(ss, 1.0f / (8 * LPR), eps), r = rsqrtf(m);
+  // a root outside [2^-50, 2^50]: its squares may have left the range of 32 bits. The row times a power of two
+  const bool far = norm && __float_as_uint(r) - __float_as_uint(0x1p-50f) > __float_as_uint(0x1p50f) - __float_as_uint(0x1p-50f);
+  if (__any_sync(0xffffffffu, far)) {
+    const float s = !far ? 1.0f : m > 1.0f ? 0x1p-100f : 0x1p100f;
+    ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] *= s, ss = fmaf(x[i], x[i], ss);
+#pragma unroll
+    for (int o = LPR / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    m = fmaf(ss, 1.0f / (8 * LPR), eps * s * s);
     r = rsqrtf(m);
-    r = fmaf(0.5f * r, fmaf(-m * r, r, 1.0f), r);  // a Newton step: its two units in the last place become one half
-    if (!(r < INFINITY)) r = rsqrtf(m);            // (zero and infinite m)
+    if (m == INFINITY) m = 0.f;  // r is 0 and stays it
   }
+  r = norm ? fmaf(0.5f * r, fmaf(-m * r, r, 1.0f), r) : 1.0f;  // a Newton step: two units in the last place become one half
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = x[i] * r * w[i];
   if (half == 0) return;
