@@ -149,48 +149,53 @@ struct Run {   // a CTA's run of units
 
 // The whole CTA: finds its run. sums: THREADS / 32 elements of shared memory.
 template <int R, int TILE, int OV, int THREADS>
-__device__ __forceinline__ Run find_run(const AttnParams& p, int64_t* sums, Run* found) {
+__device__ __forceinline__ Run find_run(const AttnParams& p, uint2* sums, Run* found) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int n_u = p.b.n_seq * p.n_qt;
   const int per = (n_u + THREADS - 1) / THREADS;
   const int u0 = min((int64_t)n_u, (int64_t)per * tid), u1 = min((int64_t)n_u, (int64_t)u0 + per);
-  int64_t incl = 0, mine;
+  int64_t own = 0;
   for (int u = u0; u < u1; ++u) {
     const int t = item_of<R, TILE>(p, u).tiles;
-    if (t) incl += p.whole ? 1 : t + OV;
+    if (t) own += p.whole ? 1 : t + OV;
   }
-  mine = incl;
+  const uint32_t mine = (uint32_t)own;
+  uint32_t incl = mine;  // sums modulo 2^32, and beside them the sum of what lies above 16 bits
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+    const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += v;
   }
-  if (lane == 31) sums[warp] = incl;
+  const uint32_t above = __reduce_add_sync(0xffffffffu, (uint32_t)min(own >> 16, (int64_t)1 << 20));
+  if (lane == 31) sums[warp] = make_uint2(incl, above);
   if (tid == 0) found->left = 0;
   __syncthreads();
-  int64_t before = incl - mine, all = 0;
+  uint32_t before_u = incl - mine, all = 0, high = 0;
   for (int w = 0; w < THREADS / 32; ++w) {
-    if (w < warp) before += sums[w];
-    all += sums[w];
+    const uint2 v = sums[w];
+    if (w < warp) before_u += v.x;
+    all += v.x;
+    high += v.y;
   }
   const int heads = p.pg.n_head_kv;
-  if (all * heads > INT32_MAX) {  // the whole grid alike: no runs
+  // high < 2^15: the sum is below 2^31 + THREADS * 2^16, so `all` is exact
+  if (high >> 15 || (uint64_t)all * heads > INT32_MAX) {  // the whole grid alike: no runs
     if (tid == 0) kv_report(p.pg.err, DMOE_KV_ERR_BATCH);
     all = 0;
   }
   const int total = (int)(all * heads);
+  int before = (int)(before_u * heads);  // in range wherever there is a run
   const int chunk = (int)(((uint32_t)total + gridDim.x - 1) / gridDim.x);
   const int first = (int)min((int64_t)chunk * blockIdx.x, (int64_t)total);
-  before *= heads;  // in range wherever there is a run
-  if (first < total && first >= before && first < before + mine * heads) {
+  if (first < total && first >= before && first < before + (int)mine * heads) {
     for (int u = u0; u < u1; ++u) {
       const Item it = item_of<R, TILE>(p, u);
       const int w = !it.tiles ? 0 : p.whole ? 1 : it.tiles + OV;
       if (first < before + w * heads) {
         found->it = it;
         found->u = u;
-        found->head = (int)(first - before) / w;
-        found->unit = (int)(first - before) % w;
+        found->head = (first - before) / w;
+        found->unit = (first - before) % w;
         found->left = min(chunk, total - first);
         break;
       }
@@ -407,7 +412,7 @@ __global__ void __launch_bounds__(32 * RowsCfg<HD, KV, NT>::kWarps, 1) kv_rows_k
   constexpr int VW = VB / 4;
   constexpr int JT = HD / 16;              // 16-row tiles of o^T
   extern __shared__ __align__(128) float smem_f[];
-  __shared__ int64_t sums[C::kWarps];
+  __shared__ uint2 sums[C::kWarps];
   __shared__ Run found;
   __shared__ uint64_t bar[C::kWarps][C::kStages];  // a stage's copies have arrived
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
@@ -806,7 +811,7 @@ __global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__
   extern __shared__ uint8_t smem_raw[];
   __shared__ TileBars bar;
   __shared__ uint32_t tmem_base_s;
-  __shared__ int64_t sums[C::kThreads / 32];
+  __shared__ uint2 sums[C::kThreads / 32];
   __shared__ Run found;
   // [item of the run & 3][sign][d]: first position whose value is +inf, or -inf; both for NaN
   __shared__ int not_finite_from[4][2][HD];
