@@ -34,7 +34,7 @@ namespace dmoe {
 namespace {
 
 constexpr int kMaxGrid = 148;  // one CTA an SM
-// The least factor of a score. Operands are at most 1 (queries) and 65504, so below it no score counts
+// The least factor of a score. Operands are at most 4 (queries) and 65504, so below it no score counts
 constexpr float kTinyFactor = 0x1p-126f;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -503,8 +503,8 @@ __global__ void __launch_bounds__(32 * RowsCfg<HD, KV, NT>::kWarps, 1) kv_rows_k
       }
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-      // f16 products: rows scaled into [-1, 1]
-      const int e = kBf ? 0 : min(max((int)(__float_as_uint(amax) >> 23) - 126, -100), 100);
+      // f16 products: rows scaled into [-1, 1] (past 2^126, where 2^e must stay a float, into [-4, 4])
+      const int e = kBf ? 0 : min(max((int)(__float_as_uint(amax) >> 23) - 126, -100), 126);
       const float inv = pow2i(-e);
 #pragma unroll
       for (int k = 0; k < HD / 16; ++k) {
@@ -1172,9 +1172,10 @@ __global__ void __launch_bounds__(640, 1) kv_tile_kernel(const __grid_constant__
             }
             a = max(a & 0xffffu, a >> 16);
             const float amax = p.is_bf16 ? __uint_as_float(a << 16) : __half2float(__ushort_as_half((uint16_t)a));
-            const int e = min(max((int)(__float_as_uint(amax) >> 23) - 126, -100), 100);
+            const int e = min(max((int)(__float_as_uint(amax) >> 23) - 126, -100), 126);
             inv = pow2i(-e);
-            factor = fmaxf(factor * pow2i(e), kTinyFactor);
+            factor *= pow2i(e);
+            if (KV != KV_E4M3) factor = fmaxf(factor, kTinyFactor);  // 8-bit pages: when the keys' scale is in it
           }
 #pragma unroll 2
           for (int i = 0; i < HD / 8; ++i) {
