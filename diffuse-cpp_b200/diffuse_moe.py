@@ -706,13 +706,14 @@ class PagedKV:
         ws = self._empty(self.err, (size // 4,), None, given)
         return self._lib.dmoe_kv_attention(cache, batch._ref, args, ws.data_ptr(), size, stream)
 
-    def check(self) -> None:
-        """Waits for the device and raises if a kernel met a page number or a batch entry out of its bounds
-        since the last check (such entries are skipped, see include/diffuse_moe.h)."""
+    def check(self, all_streams: bool = True) -> None:
+        """Waits for the device (all_streams=False: for the current stream alone, where that has all the calls) and
+        raises if a kernel met a page number or a batch entry out of its bounds since the last check (such
+        entries are skipped, see include/diffuse_moe.h)."""
         import torch
 
-        if self.err.is_cuda:
-            torch.cuda.synchronize(self.device)  # calls on every stream, not the current one alone
+        if all_streams and self.err.is_cuda:
+            torch.cuda.synchronize(self.device)
         bits = int(self.err.item())
         if bits:
             self.err.zero_()

@@ -468,7 +468,8 @@ def generate_batch(model: LLaDA2Model, prompts: list, n_generate: int, steps: in
     report = getattr(kv, "check", None)  # a stand-in without kernels has no error word
     while True:
         if report is not None:
-            report()  # attention that is not complete, or that read wrong pages, ends the generation
+            # attention that is not complete, or that read wrong pages, ends the generation. Its calls are on this stream
+            report(all_streams=False)
         live = [i for i in range(len(prompts)) if blk[i] < n_blocks[i] and step[i] < len(sched)]
         if not live:
             return [s.cpu().numpy() for s in seqs], forwards

@@ -22,7 +22,7 @@ class Reporting(Pages):
             self.bits = 4
         return super().attend(*a, **k)
 
-    def check(self):
+    def check(self, all_streams=True):
         if self.bits:
             self.bits = 0
             raise dm.DmoeError(6, "paged cache: a device-side wait timed out")
