@@ -18,10 +18,11 @@
 // until its amax is known. 16 lanes (head_dim 128) or 8 (64) share a row, 8 elements each: 16-byte
 // loads of 16-bit rows, two or four rows a warp at once, and half the shuffles of a warp per row.
 //
-// Measured on B200 (32 + 4 + 4 heads of 128, rotary_dim 64, e4m3): a 16384-token prompt, 318.8 MB, 118 us = 2.7 TB/s, 42 %
-// of the copy rate (101 us with keys in 32 bits). Instruction issue bounds it, not HBM: norm, rotation and conversion
+// Measured on B200 (32 + 4 + 4 heads of 128, rotary_dim 64, e4m3): a 16384-token prompt, 318.8 MB, 120 us = 2.7 TB/s, 41 %
+// of the copy rate (17 us less with keys in 32 bits). Instruction issue bounds it, not HBM: norm, rotation and conversion
 // take about 150 instructions per 8 elements. One block of 32 positions: 10 us a call, most of it the launch and
-// the host.
+// the host. Many single tokens: every warp scans the batch for its unit, which takes most of the time beyond some hundreds
+// of sequences (1024: 102 us, 4096: 786 us).
 #include <algorithm>
 #include <cmath>
 #include <cstdio>
@@ -37,8 +38,10 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxHalf = 64;  // rotary_dim / 2 at head_dim 128
-constexpr int kWantedHeld = 148 * 3;  // of them for the keys of 8-bit pages, whose table is dearer
-constexpr int kWanted = 148 * 6;  // CTAs of a large call (16384-token prompt: 125 us at 6 an SM, 134 at 12, 161 at 24)
+constexpr int kWantedHeld = 148 * 3;  // of them for the keys of 8-bit pages, whose table is dearer (prompt: 123 us at 6 an SM)
+// CTAs of a large call (16384-token prompt: 119 us at 4 or 6 an SM, 128 at 12, 139 at 24; 24 x 64 rows into bf16 pages:
+// 21.2, 20.7, 23.0, 32.8)
+constexpr int kWanted = 148 * 6;
 
 struct AppendParams {
   KvPages pg;

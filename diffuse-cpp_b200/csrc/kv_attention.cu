@@ -383,7 +383,7 @@ __device__ __forceinline__ void store_lse(const AttnParams& p, int row0, int row
 // has them brought into shared memory by one bulk copy each, one or two steps ahead (no barrier but the copies' own), so
 // that the latency of HBM does not show. A step's chain of dependent instructions is long, and only other warps
 // hide it: as many as registers and the ring leave room for. Measured: 64 tokens over 545 K positions of e4m3
-// pages (558 MB) 105 us = 5.3 TB/s, 82 % of the copy rate; one token over 131072 positions 37 us with the second kernel.
+// pages (558 MB) 108 us = 5.2 TB/s, 80 % of the copy rate; one token over 131072 positions 37 us with the second kernel.
 // ---------------------------------------------------------------------------------------------
 template <int HD, int KV, int NT>
 struct RowsCfg {
@@ -778,8 +778,9 @@ __global__ void __launch_bounds__(32 * RowsCfg<HD, KV, NT>::kWarps, 1) kv_rows_k
 // then.
 // Bound by a half's chain of scores (512 cycles of the tensor pipe), exponentials (128 a thread, 8 cycles a warp:
 // 1024 at least) and products (512), of which two are in flight: about 3800 cycles for two tiles. Measured: 2048 rows
-// over 16384 positions of bf16 pages 530 us = 0.98 PFLOP/s (tensor pipe 55 % active, exponential unit 55 %); 16
-// blocks of 32 rows over 0.5-16 K positions of e4m3 pages 118 us; a prompt of 4096 230 us.
+// over 16384 positions of bf16 pages 535 us = 0.97 PFLOP/s (tensor pipe 54 % active, exponential unit 54 %); 16
+// blocks of 32 rows over 0.5-16 K positions of e4m3 pages 117 us; a prompt of 4096 230 us. The registers of every
+// role spill (1.4 KB of stores a thread): run, walk and item are carried by all of them.
 // ---------------------------------------------------------------------------------------------
 template <int HD, int KV>
 struct TileCfg {
